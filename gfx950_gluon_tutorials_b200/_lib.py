@@ -22,6 +22,7 @@ EINVAL, ESHAPE, EALIGN, ESTRIDE, EWORKSPACE, ETENSORMAP, ENODEVICE, ECAPACITY = 
 STATUS_TIMEOUT = 0x1000
 STATUS_SMEM_BASE = 0x2000
 STATUS_BAD_GROUPS = 0x3000
+STATUS_PAGE_TABLE, STATUS_SLOT, STATUS_TOKENS = 0x4000, 0x5000, 0x6000
 SITE_EMPTY, SITE_FULL, SITE_ACC_EMPTY, SITE_ACC_FULL, SITE_OVERLAP, SITE_FLAG = 1, 2, 3, 4, 5, 6
 SITE_SCALES = 7
 OPT_PAIR, OPT_SK_MODE, OPT_GROUP_M, OPT_MIN_SK_ITERS, OPT_TIMEOUT_MS = 1, 2, 3, 4, 5
@@ -57,6 +58,19 @@ SIGNATURES = {
     "b2g_attention_fwd": (_c_int, [_vp, _vp, _vp, _vp, ctypes.POINTER(ctypes.c_int64), _c_int,
                                    _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                    ctypes.c_float, _vp, _vp, _vp]),
+    "b2g_kv_map_step": (_c_int, [_vp, _vp, _vp, _vp, _c_i64, _c_int, _c_int, _vp, _c_i64, _vp,
+                                 _c_int, _c_i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "b2g_kv_write": (_c_int, [_vp, _vp, _vp, _vp, ctypes.POINTER(ctypes.c_int64), _vp, _c_i64,
+                              _c_int, _c_int, _c_i64, _c_int, _c_int, _vp, _vp]),
+    "b2g_attention_prefill_workspace_bytes": (_c_sz, [_c_int, _c_i64, _c_int]),
+    "b2g_attention_prefill": (_c_int, [_vp, _vp, _vp, _vp, ctypes.POINTER(ctypes.c_int64), _vp,
+                                       _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int,
+                                       ctypes.c_float, _vp, _vp, _c_sz, _vp, _vp]),
+    "b2g_attention_tree_workspace_bytes": (_c_sz, [_c_int, _c_i64, _c_int, _c_int, _c_int]),
+    "b2g_attention_tree": (_c_int, [_vp, _vp, _vp, _vp, ctypes.POINTER(ctypes.c_int64), _vp,
+                                    _c_i64, _c_int, _vp, _vp, _vp, _c_int, _c_int, _c_i64, _c_int,
+                                    _c_int, _c_int, _c_i64, _c_int, _c_int, ctypes.c_float, _vp,
+                                    _vp, _c_sz, _vp, _vp]),
     "b2g_selftest_poly_exp2": (_c_int, [_vp, _vp, _vp, _vp, _c_i64, _vp]),
     "b2g_gemm_mxf4_noalloc": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _vp,
                                        _c_i64, _c_i64, _vp, _c_i64, _c_int, _c_int, _c_int,

@@ -13,7 +13,11 @@ differ and need not be multiples of 64 (rows and keys past the ends are
 masked), and the softmax log-sum-exp can be returned. ``scale_on_q`` is
 accepted for signature compatibility; the kernel always applies the scale to
 the fp32 scores, which is the more accurate of the reference's two choices.
-Causal masking is not supported, as in the reference tutorial kernel.
+Causal masking is not supported there, as in the reference tutorial kernel.
+
+``attention_prefill`` (causal, packed prompts) and ``attention_tree`` (drafted or
+single tokens over a paged cache, see ``kvcache``) are a serving step's
+attention; the reference has no counterpart.
 """
 
 from __future__ import annotations
@@ -24,7 +28,8 @@ import math
 import torch
 
 from . import _lib
-from .ops import _require_cuda, _stream_handle, status_tensor
+from .kvcache import _int_vector, check_caches
+from .ops import _require_cuda, _stream_handle, status_tensor, workspace
 
 _DT = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
 HEAD_DIMS = (64, 128)
@@ -166,6 +171,150 @@ def run_gluon_attention(q, k, v, o, metadata: MetaData, scale_on_q: bool = True)
     assert nheads_q % nheads_k == 0, "query heads must be a multiple of key/value heads"
     del scale_on_q  # the scale is always applied to the fp32 scores
     return attention_fwd(q, k, v, o, sm_scale=metadata.sm_scale, layout=metadata.layout)
+
+
+def _packed(t: torch.Tensor) -> bool:
+    """Whether a (tokens, heads, dim) tensor can be read or written where it lies: unit
+    dim stride, 16-byte aligned base and rows."""
+    s0, s1, s2 = t.stride()
+    return s2 == 1 and s0 > 0 and s1 > 0 and not ((s0 | s1) & 7) and not t.data_ptr() & 15
+
+
+def _readable(t: torch.Tensor) -> torch.Tensor:
+    return t if _packed(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def _check_packed(q: torch.Tensor, hk: int, o, lse) -> tuple[int, int, int, torch.Tensor]:
+    """Shapes of q, its output and its lse; returns (tokens, heads, dim, o)."""
+    if q.dtype not in _DT:
+        raise ValueError("q must be float16 or bfloat16")
+    tokens, hq, dim = q.shape
+    if dim not in HEAD_DIMS:
+        raise ValueError(f"head dim must be one of {HEAD_DIMS}, got {dim}")
+    if hk < 1 or hq % hk:
+        raise ValueError("query heads must be a multiple of key/value heads")
+    if o is None:
+        o = torch.empty((tokens, hq, dim), dtype=q.dtype, device=q.device)
+    elif o.shape != q.shape or o.dtype != q.dtype:
+        raise ValueError("o must have q's shape and dtype")
+    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (hq, tokens)
+                            or not lse.is_contiguous()):
+        raise ValueError(f"lse must be a contiguous float32 ({hq}, {tokens}) tensor")
+    return tokens, hq, dim, o
+
+
+def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                      o: torch.Tensor | None = None, *, sm_scale: float | None = None,
+                      lse: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention over packed prompts: token i of a prompt sees its tokens 0 .. i.
+
+    ``q`` (tokens, HQ, D), ``k`` and ``v`` (tokens, HK, D) hold the prompts back to
+    back, prompt b in rows cu_seqlens[b] .. cu_seqlens[b + 1] (int32, on the GPU;
+    empty prompts are fine). Rows past the last prompt are not written. ``lse``, if
+    given, is a float32 (HQ, tokens) tensor that receives the natural-log
+    log-sum-exp of each row's scaled scores. D is 64 or 128. Asynchronous on the
+    current stream; offsets that decrease or pass ``tokens`` and kernel timeouts
+    are reported by ``ops.check_status``.
+    """
+    dev = _require_cuda(q, k, v, cu_seqlens, o, lse)
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape:
+        raise ValueError("q, k and v must be (tokens, heads, head_dim), k and v of one shape")
+    tokens, hq, dim, o = _check_packed(q, k.shape[1], o, lse)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v must share one dtype, float16 or bfloat16")
+    if k.shape[0] != tokens or k.shape[2] != dim:
+        raise ValueError(f"k/v shape {tuple(k.shape)} does not match q {tuple(q.shape)}")
+    cu_seqlens = _int_vector(cu_seqlens, None, torch.int32, "cu_seqlens")
+    prompts = cu_seqlens.shape[0] - 1
+    if prompts < 0:
+        raise ValueError("cu_seqlens needs at least one entry")
+    if tokens == 0 or prompts == 0:
+        return o
+    q, k, v = _readable(q), _readable(k), _readable(v)
+    out = o if _packed(o) else torch.empty(o.shape, dtype=o.dtype, device=dev)
+    if out is not o:
+        out.copy_(o)  # rows past the last prompt keep what o holds
+    strides = (ctypes.c_int64 * 8)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2],
+                                   *out.stride()[:2])
+    handle = _lib.lib()
+    ws = workspace(handle.b2g_attention_prefill_workspace_bytes(prompts, tokens, hq), dev)
+    rc = handle.b2g_attention_prefill(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), strides, cu_seqlens.data_ptr(),
+        prompts, tokens, hq, k.shape[1], dim, _DT[q.dtype],
+        dim ** -0.5 if sm_scale is None else sm_scale, None if lse is None else lse.data_ptr(),
+        ws.data_ptr(), ws.numel(), status_tensor(dev).data_ptr(), _stream_handle(dev))
+    _lib.check(rc, "b2g_attention_prefill")
+    if out is not o:
+        o.copy_(out)
+    return o
+
+
+def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   block_tables: torch.Tensor, seq_lens: torch.Tensor, cu_seqlens: torch.Tensor,
+                   tree_mask: torch.Tensor | None = None, o: torch.Tensor | None = None, *,
+                   sm_scale: float | None = None, lse: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a step's new tokens over a paged cache that already holds them.
+
+    ``q`` (tokens, HQ, D) packs the requests' new tokens, request r's in rows
+    cu_seqlens[r] .. cu_seqlens[r + 1]; they are the last tokens of the seq_lens[r]
+    that the cache holds for it in the pages of row r of ``block_tables``. A new
+    token sees every older token of its request, and of the new ones those whose
+    bit is set in its row of ``tree_mask`` (int64 (tokens, words); bit j % 64 of
+    word j // 64 is the request's new token j, and a token sets its own bit too).
+    Without a mask the new tokens are a chain, each seeing the ones before it: one
+    token per request is plain decoding, many are a chunk of a prompt. A token that
+    sees nothing gets zeros and an lse of -inf.
+
+    The caches are (pages, page_size, HK, D) with unit dim stride, 16-byte aligned
+    rows and a page_size of 8, 16, 32, 64 or a multiple of 128; they are never
+    copied. ``block_tables`` is int32 (requests, max_pages), ``seq_lens`` and
+    ``cu_seqlens`` int32, ``lse`` as for ``attention_prefill``. Asynchronous on the
+    current stream; bad pages and lengths are reported by ``ops.check_status``.
+    """
+    dev = _require_cuda(q, k_cache, v_cache, block_tables, seq_lens, cu_seqlens, tree_mask, o, lse)
+    if q.dim() != 3:
+        raise ValueError("q must be (tokens, heads, head_dim)")
+    check_caches(k_cache, v_cache, q.dtype)
+    pages, page, hk, cache_dim = k_cache.shape
+    tokens, hq, dim, o = _check_packed(q, hk, o, lse)
+    if cache_dim != dim:
+        raise ValueError(f"q has heads of {dim}, the cache of {cache_dim}")
+    if block_tables.dim() != 2 or block_tables.dtype != torch.int32:
+        raise ValueError("block_tables must be a 2-D int32 tensor")
+    requests, max_pages = block_tables.shape
+    if max_pages > 1 and block_tables.stride(1) != 1:
+        block_tables = block_tables.contiguous()
+    seq_lens = _int_vector(seq_lens, requests, torch.int32, "seq_lens")
+    cu_seqlens = _int_vector(cu_seqlens, requests + 1, torch.int32, "cu_seqlens")
+    words = 0
+    if tree_mask is not None:
+        if tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != tokens:
+            raise ValueError(f"tree_mask must be an int64 ({tokens}, words) tensor")
+        words = tree_mask.shape[1]
+        if words < 1:
+            raise ValueError("tree_mask needs at least one word per token")
+        tree_mask = tree_mask.contiguous()
+    if tokens == 0 or requests == 0:
+        return o
+    q = _readable(q)
+    out = o if _packed(o) else torch.empty(o.shape, dtype=o.dtype, device=dev)
+    if out is not o:
+        out.copy_(o)  # rows past the last request keep what o holds
+    strides = (ctypes.c_int64 * 10)(*q.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3],
+                                    *out.stride()[:2])
+    handle = _lib.lib()
+    ws = workspace(handle.b2g_attention_tree_workspace_bytes(requests, tokens, hq, hk, dim), dev)
+    rc = handle.b2g_attention_tree(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), strides,
+        block_tables.data_ptr(), block_tables.stride(0), max_pages, seq_lens.data_ptr(),
+        cu_seqlens.data_ptr(), None if tree_mask is None else tree_mask.data_ptr(), words,
+        requests, tokens, hq, hk, dim, pages, page, _DT[q.dtype],
+        dim ** -0.5 if sm_scale is None else sm_scale, None if lse is None else lse.data_ptr(),
+        ws.data_ptr(), ws.numel(), status_tensor(dev).data_ptr(), _stream_handle(dev))
+    _lib.check(rc, "b2g_attention_tree")
+    if out is not o:
+        o.copy_(out)
+    return o
 
 
 def main(argv=None) -> None:

@@ -713,6 +713,10 @@ const char* b2g_strerror(int code) {
     case B2G_STATUS_BAD_GROUPS:
       return "grouped GEMM refused to run: group offsets must start at 0, end at M, not "
              "decrease and be multiples of the tile height";
+    case B2G_STATUS_PAGE_TABLE:
+      return "a block table names a page outside the cache or has too few columns";
+    case B2G_STATUS_SLOT: return "a slot lies past the end of the cache";
+    case B2G_STATUS_TOKENS: return "the lengths add up to more tokens than the call has";
     case B2G_STATUS_SMEM_BASE:
       return "kernel refused to run: dynamic shared memory base needs more alignment padding "
              "than was reserved";

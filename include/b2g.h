@@ -85,6 +85,9 @@ extern "C" {
 #define B2G_SITE_SCALES 7         /* MMA waiting for scale factors copied into TMEM */
 #define B2G_STATUS_SMEM_BASE 0x2000 /* kernel returned at entry: shared memory base misaligned */
 #define B2G_STATUS_BAD_GROUPS 0x3000 /* grouped GEMM returned at entry: group offsets invalid */
+#define B2G_STATUS_PAGE_TABLE 0x4000 /* a block table names a page outside the cache, or has too few columns */
+#define B2G_STATUS_SLOT 0x5000       /* a slot lies past the end of the cache; nothing was stored there */
+#define B2G_STATUS_TOKENS 0x6000     /* the lengths add up to more tokens than the call has */
 
 /* Library ABI version (major * 100 + minor). */
 B2G_API int b2g_version(void);
@@ -225,6 +228,91 @@ B2G_API int b2g_attention_fwd(const void* q, const void* k, const void* v, void*
                               const int64_t* strides, int batch, int heads_q, int heads_k,
                               int seqlen_q, int seqlen_k, int head_dim, int dtype,
                               float sm_scale, float* lse, int* status, void* stream);
+
+/* ---- serving: a paged key/value cache and the attention over it ----
+ * A cache is a pair of tensors of `num_pages` pages of `page_size` token slots
+ * each, per slot `heads_k` rows of `head_dim` elements; slot s is row s %
+ * page_size of page s / page_size. A request's block table lists its pages in
+ * order. Tokens of a step are packed: request r's are rows cu_seqlens[r] ..
+ * cu_seqlens[r + 1] of every per-token tensor. Lengths, tables, slots and masks
+ * are device arrays; nothing here reads them on the host. These entry points
+ * have no counterpart in the reference, whose attention is dense. */
+
+/* Block tables and slot maps from request lengths, in one launch. Request r has
+ * cached_lens[r] tokens in the cache, page_counts[r] valid entries in row r of
+ * block_tables (row stride `table_stride`, `max_pages` columns) and new_lens[r]
+ * new tokens. The pages that it lacks for cached + new tokens are taken from
+ * the top of the stack free_pages[0 .. *num_free), request by request, and
+ * appended to its row. Written: slots and positions of the `num_tokens` packed
+ * new tokens (rows past the last token: slot -1, position 0), cu_seqlens
+ * (requests + 1), seq_lens = cached + new, page_counts_out and num_free_out.
+ * When the list runs out, the missing table entries and their tokens' slots are
+ * -1 and num_free_out is minus the number of missing pages. Inputs other than
+ * block_tables are not changed (the outputs may not alias them), so a call can
+ * be repeated. Negative lengths count as 0. Status: B2G_STATUS_PAGE_TABLE when
+ * a request outgrows max_pages (the tokens past it get slot -1),
+ * B2G_STATUS_TOKENS when there are more than num_tokens new tokens (cu_seqlens
+ * is cut there). At most 8192 requests (else B2G_ECAPACITY). */
+B2G_API int b2g_kv_map_step(const int32_t* cached_lens, const int32_t* new_lens,
+                            const int32_t* page_counts, int32_t* block_tables,
+                            int64_t table_stride, int requests, int max_pages,
+                            const int32_t* free_pages, int64_t free_capacity,
+                            const int32_t* num_free, int page_size, int64_t num_tokens,
+                            int64_t* slots, int32_t* positions, int32_t* cu_seqlens,
+                            int32_t* seq_lens, int32_t* page_counts_out, int32_t* num_free_out,
+                            int* status, void* stream);
+
+/* Stores k and v rows (tokens x heads x head_dim, fp16 or bf16, dim stride 1)
+ * at slots[token] of the caches. `strides` holds 10 element strides: k (token,
+ * head), v (token, head), k_cache (page, slot, head), v_cache (page, slot,
+ * head). Any alignment (16-byte aligned rows are fastest). Negative slots are
+ * skipped; a slot past the cache sets B2G_STATUS_SLOT and is skipped. Two
+ * tokens with one slot leave either's row there. */
+B2G_API int b2g_kv_write(const void* k, const void* v, void* k_cache, void* v_cache,
+                         const int64_t* strides, const int64_t* slots, int64_t tokens, int heads,
+                         int head_dim, int64_t num_pages, int page_size, int dtype, int* status,
+                         void* stream);
+
+/* Causal attention over packed prompts with grouped-query heads: token i of a
+ * prompt sees the prompt's tokens 0 .. i. `strides` holds 8 element strides,
+ * (token, head) of q, k, v, o; the dim stride is 1, the others positive
+ * multiples of 8, pointers 16-byte aligned. Prompts may be empty; rows of o and
+ * lse past cu_seqlens[prompts] are not written. Offsets that decrease or pass
+ * `tokens` are clamped and set B2G_STATUS_TOKENS. lse (nullable) is float
+ * [heads_q][tokens]. Workspace as for the GEMMs, of at least
+ * b2g_attention_prefill_workspace_bytes(prompts, tokens, heads_q) bytes. */
+B2G_API size_t b2g_attention_prefill_workspace_bytes(int prompts, int64_t tokens, int heads_q);
+B2G_API int b2g_attention_prefill(const void* q, const void* k, const void* v, void* o,
+                                  const int64_t* strides, const int32_t* cu_seqlens, int prompts,
+                                  int64_t tokens, int heads_q, int heads_k, int head_dim,
+                                  int dtype, float sm_scale, float* lse, void* workspace,
+                                  size_t workspace_bytes, int* status, void* stream);
+
+/* Attention of a step's new tokens over the paged cache, which already holds
+ * their keys and values: request r has seq_lens[r] tokens in all, of which the
+ * last n_r = cu_seqlens[r + 1] - cu_seqlens[r] are the step's. Its new token i
+ * sees every older token, and new token j where bit j % 64 of
+ * tree_mask[token * mask_words + j / 64] is set (an ancestor mask, its own bit
+ * included); with tree_mask null the new tokens are a chain (j <= i), which for
+ * n_r = 1 is plain decoding. A token that sees nothing gets zeros and an lse of
+ * -inf. `strides` holds 10 element strides: q (token, head), k_cache (page,
+ * slot, head), v_cache (page, slot, head), o (token, head); dim stride 1, the
+ * others positive multiples of 8, pointers 16-byte aligned. page_size 8, 16, 32,
+ * 64 or a multiple of 128. Keys in a page past seq_lens[r] are never used,
+ * whatever they hold. A table entry outside [0, num_pages) reads as zero keys
+ * and values and sets B2G_STATUS_PAGE_TABLE, as does a request longer than its
+ * table. lse (nullable) is float [heads_q][tokens]. Workspace as for the GEMMs,
+ * of at least b2g_attention_tree_workspace_bytes(...) bytes. */
+B2G_API size_t b2g_attention_tree_workspace_bytes(int requests, int64_t tokens, int heads_q,
+                                                  int heads_k, int head_dim);
+B2G_API int b2g_attention_tree(const void* q, const void* k_cache, const void* v_cache, void* o,
+                               const int64_t* strides, const int32_t* block_tables,
+                               int64_t table_stride, int max_pages, const int32_t* seq_lens,
+                               const int32_t* cu_seqlens, const int64_t* tree_mask,
+                               int mask_words, int requests, int64_t tokens, int heads_q,
+                               int heads_k, int head_dim, int64_t num_pages, int page_size,
+                               int dtype, float sm_scale, float* lse, void* workspace,
+                               size_t workspace_bytes, int* status, void* stream);
 
 /* Diagnostic, no counterpart in the reference: evaluates the FMHA's FMA-pipe
  * exponential (a cubic for 2^f, f in [-0.5, 0.5], plus an exponent-field add;
