@@ -123,55 +123,11 @@ int launch_rows(const RowsParams& p, int head_dim, int dtype, cudaStream_t s) {
   return e == cudaSuccess ? B2G_OK : static_cast<int>(e);
 }
 
-// Shared checks of the two entry points; strides: n of them, all positive multiples of 8.
-int check_attention(int heads_q, int heads_k, int head_dim, int dtype, float sm_scale,
-                    const int64_t* strides, int n, std::initializer_list<const void*> ptrs) {
-  if (strides == nullptr) return B2G_EINVAL;
-  if (dtype != B2G_DT_F16 && dtype != B2G_DT_BF16) return B2G_EINVAL;
-  if (!(sm_scale > 0.0f) || !std::isfinite(sm_scale)) return B2G_EINVAL;
-  if (head_dim != 64 && head_dim != 128) return B2G_ESHAPE;
-  if (heads_q < 1 || heads_k < 1 || heads_q % heads_k != 0 || heads_q > 65535) return B2G_ESHAPE;
-  for (const void* ptr : ptrs)
-    if (ptr == nullptr) return B2G_EINVAL;
-  for (int i = 0; i < n; ++i)
-    if (strides[i] <= 0) return B2G_ESTRIDE;
-  for (int i = 0; i < n; ++i)
-    if (strides[i] % 8 != 0) return B2G_EALIGN;
-  for (const void* ptr : ptrs)
-    if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0) return B2G_EALIGN;
-  return B2G_OK;
-}
 }  // namespace
 
 }  // namespace b2g
 
-extern "C" size_t b2g_attention_prefill_workspace_bytes(int, int64_t, int) { return 0; }
 extern "C" size_t b2g_attention_tree_workspace_bytes(int, int64_t, int, int, int) { return 0; }
-
-extern "C" int b2g_attention_prefill(const void* q, const void* k, const void* v, void* o,
-                                     const int64_t* strides, const int32_t* cu_seqlens,
-                                     int prompts, int64_t tokens, int heads_q, int heads_k,
-                                     int head_dim, int dtype, float sm_scale, float* lse,
-                                     void* workspace, size_t workspace_bytes, int* status,
-                                     void* stream) {
-  using namespace b2g;
-  if (tokens < 0 || tokens > INT_MAX - 256 || prompts < 0) return B2G_ESHAPE;
-  if (tokens == 0 || prompts == 0) return B2G_OK;
-  const int rc = check_attention(heads_q, heads_k, head_dim, dtype, sm_scale, strides, 8, {q, k, v, o});
-  if (rc != B2G_OK) return rc;
-  if (cu_seqlens == nullptr) return B2G_EINVAL;
-  if (current_device_sms() <= 0) return B2G_ENODEVICE;
-  RowsParams p = {};
-  p.q = q; p.k = k; p.v = v; p.o = o;
-  p.q_t = strides[0]; p.q_h = strides[1];
-  p.k_t = strides[2]; p.k_h = strides[3];
-  p.v_t = strides[4]; p.v_h = strides[5];
-  p.o_t = strides[6]; p.o_h = strides[7];
-  p.cu = cu_seqlens; p.lse = lse; p.status = status;
-  p.requests = prompts; p.tokens = static_cast<int32_t>(tokens); p.HQ = heads_q; p.HK = heads_k;
-  p.scale = sm_scale; p.page_size = 1;
-  return launch_rows(p, head_dim, dtype, static_cast<cudaStream_t>(stream));
-}
 
 extern "C" int b2g_attention_tree(const void* q, const void* k_cache, const void* v_cache, void* o,
                                   const int64_t* strides, const int32_t* block_tables,
@@ -184,7 +140,7 @@ extern "C" int b2g_attention_tree(const void* q, const void* k_cache, const void
   using namespace b2g;
   if (tokens < 0 || tokens > INT_MAX - 256 || requests < 0) return B2G_ESHAPE;
   if (tokens == 0 || requests == 0) return B2G_OK;
-  const int rc = check_attention(heads_q, heads_k, head_dim, dtype, sm_scale, strides, 10,
+  const int rc = check_serving_attention(heads_q, heads_k, head_dim, dtype, sm_scale, strides, 10,
                                  {q, k_cache, v_cache, o});
   if (rc != B2G_OK) return rc;
   if (block_tables == nullptr || seq_lens == nullptr || cu_seqlens == nullptr) return B2G_EINVAL;

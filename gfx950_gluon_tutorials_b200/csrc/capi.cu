@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdint>
 #include <cstring>
 #include <mutex>
@@ -671,6 +672,27 @@ int gemm_mxf4_fixed_scratch(const uint8_t* A, int64_t lda, const uint8_t* B, int
 
 
 int current_device_sms() { return current_sms(); }
+
+size_t workspace_flag_bytes(int sms) { return flag_region_bytes(sms); }
+
+int check_serving_attention(int heads_q, int heads_k, int head_dim, int dtype, float sm_scale,
+                            const int64_t* strides, int n,
+                            std::initializer_list<const void*> ptrs) {
+  if (strides == nullptr) return B2G_EINVAL;
+  if (dtype != B2G_DT_F16 && dtype != B2G_DT_BF16) return B2G_EINVAL;
+  if (!(sm_scale > 0.0f) || !std::isfinite(sm_scale)) return B2G_EINVAL;
+  if (head_dim != 64 && head_dim != 128) return B2G_ESHAPE;
+  if (heads_q < 1 || heads_k < 1 || heads_q % heads_k != 0 || heads_q > 65535) return B2G_ESHAPE;
+  for (const void* ptr : ptrs)
+    if (ptr == nullptr) return B2G_EINVAL;
+  for (int i = 0; i < n; ++i)
+    if (strides[i] <= 0) return B2G_ESTRIDE;
+  for (int i = 0; i < n; ++i)
+    if (strides[i] % 8 != 0) return B2G_EALIGN;
+  for (const void* ptr : ptrs)
+    if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0) return B2G_EALIGN;
+  return B2G_OK;
+}
 
 PFN_cuTensorMapEncodeTiled_v12000 tma_encoder() { return tensor_map_encoder(); }
 

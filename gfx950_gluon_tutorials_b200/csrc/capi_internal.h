@@ -8,6 +8,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <initializer_list>
 
 namespace b2g {
 
@@ -26,6 +27,15 @@ int current_device_sms();
 
 // cuTensorMapEncodeTiled from the driver, or null.
 PFN_cuTensorMapEncodeTiled_v12000 tma_encoder();
+
+// Bytes of the flag words, zero at rest, that every workspace starts with.
+size_t workspace_flag_bytes(int sms);
+
+// Argument checks that the serving attention entry points share; `strides`
+// holds `n` element strides.
+int check_serving_attention(int heads_q, int heads_k, int head_dim, int dtype, float sm_scale,
+                            const int64_t* strides, int n,
+                            std::initializer_list<const void*> pointers);
 
 // The bounded-wait limit (B2G_OPT_TIMEOUT_MS) in nanoseconds.
 uint64_t wait_timeout_ns();
