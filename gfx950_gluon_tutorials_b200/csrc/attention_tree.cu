@@ -10,7 +10,9 @@
 //
 // Work. A block's keys are tiles of 128; the tiles of all blocks, in order of
 // (block, head, tile), are one list that is cut into equal shares, one per CTA
-// (one per SM). So a batch of uneven lengths and a single long request alike keep
+// (one per SM); every CTA adds up the requests' tiles itself to find where its
+// share begins, which costs about a microsecond where a planning launch of its
+// own cost five. So a batch of uneven lengths and a single long request alike keep
 // every SM reading to the end. A block whose tiles lie in several shares is
 // joined at the end: each CTA publishes its rows of O with their maxima and sums,
 // and when all have, each joins its slice of the rows, in a fixed order.
@@ -44,19 +46,20 @@
 namespace b2g {
 
 // One row block: where it is and how many tiles its rows need.
-struct alignas(32) TreeEntry {
+struct TreeEntry {
   int32_t request, block;   // block of 256 rows of the request
   int32_t tiles;            // KV tiles, at least one
-  int32_t before;           // tiles of the blocks before this one (per key/value head)
   int32_t ctx;              // older tokens: length - new tokens (negative if it is shorter)
   int32_t fresh;            // new tokens
   int32_t first;            // first new token's row among all
   int32_t len;              // keys
 };
 
-struct TreeMeta {
-  int32_t entries, pad;
-  int64_t units;  // tiles of all blocks and key/value heads
+// Where a share begins: block `block` of request `request`, head, tile; `before`
+// units lie before the block.
+struct ShareStart {
+  int64_t units, before;
+  int32_t request, block, hk, tile;
 };
 
 struct alignas(64) TreeParams {
@@ -72,17 +75,19 @@ struct alignas(64) TreeParams {
   const int64_t* mask;
   float* lse;
   int* status;
-  const TreeEntry* plan;
-  const TreeMeta* meta;
-  const int4* start;       // per CTA: entry, head, tile of its first unit
-  float* part;             // [2 per CTA][part_rows][D] unfinished O
+  const int32_t* cu;
+  const int32_t* lens;
+  float* part;             // [2 per CTA][D / 4][part_rows] float4: unfinished O, rows side by side
   float2* part_ml;         // [2 per CTA][part_rows] {max (log2 units), sum}
   uint32_t* counters;      // two per CTA, zero at rest: published, joined
-  int32_t mask_words, part_rows;
+  int32_t mask_words, part_rows, requests;
+  int32_t most;            // keys that a table has room for
   int32_t HQ, HK, G, tokens, page_size, num_pages;
   float scale_log2;
   uint64_t timeout_ns;
 };
+
+constexpr int32_t kJoinBatch = 8;  // parts of a block that a thread reads at once
 
 template <int D>
 struct TreePlan {
@@ -93,7 +98,6 @@ struct TreePlan {
   static constexpr uint32_t kSlots = D == 128 ? 5 : 10;   // ring of K and V tiles in turn
   static constexpr uint32_t kQOff = 0;                    // two tiles
   static constexpr uint32_t kJoinOff = kTile;  // up to 128 rows the second Q tile is the join buffer
-  static constexpr uint32_t kJoinCols = D / 4; // columns joined at a time (8 warps x 32 rows x 4 B)
   static constexpr uint32_t kRingOff = 2 * kTile;
   static constexpr uint32_t kMlOff = kRingOff + kSlots * kTile;   // float2 [8 warps][32 rows]
   static constexpr uint32_t kBarOff = kMlOff + 8 * 32 * 8;
@@ -108,125 +112,122 @@ struct TreePlan {
   static constexpr uint32_t kDynBytes = kBytes + 1024 <= kMaxDyn ? kBytes + 1024 : kMaxDyn;
   static constexpr uint32_t kS = 0, kO = 256, kTileCols = 128;
   static_assert(kBytes <= kMaxDyn, "shared memory");
-  static_assert(8 * 32 * kJoinCols * 4 == kTile, "join buffer");
+  static_assert(2 * (kThreads / 32) * 8 <= 512 && 512 + sizeof(ShareStart) <= 8 * 32 * 8, "scratch");
 };
-
-// The CTA whose share holds unit u, of `ctas` equal shares of `units`.
-__device__ __forceinline__ int32_t share_of(int64_t u, int64_t units, int32_t ctas) {
-  return static_cast<int32_t>(((u + 1) * ctas - 1) / units);
-}
 
 // ------------------------------------------------------------------- plan --
-// The row blocks of all requests with running sums of their tiles, and where each
-// CTA's share begins. One CTA, latency-bound: a scan over the requests, then a
-// search per share.
-constexpr int kTreePlanThreads = 1024;
-constexpr int kTreePlanShared = 4096;  // running sums kept in shared memory for the searches
+// Request r: its new tokens and keys, cut to what the call has room for.
+__device__ __forceinline__ TreeEntry tree_request(const TreeParams& p, int32_t r, bool report) {
+  TreeEntry e;
+  const int32_t lo = p.cu[r], hi = p.cu[r + 1], len = p.lens[r];
+  e.request = r;
+  e.block = 0;
+  e.tiles = 0;
+  e.first = min(max(lo, 0), p.tokens);
+  e.fresh = min(max(hi, e.first), p.tokens) - e.first;
+  e.len = min(max(len, 0), p.most);
+  e.ctx = e.len - e.fresh;
+  if (report) {
+    if (lo < 0 || hi < lo || hi > p.tokens) fmha_report(p, B2G_STATUS_TOKENS);
+    if (len > p.most) fmha_report(p, B2G_STATUS_PAGE_TABLE);
+  }
+  return e;
+}
 
-struct TreePlanParams {
-  const int32_t* cu;
-  const int32_t* lens;
-  TreeEntry* plan;
-  TreeMeta* meta;
-  int4* start;
-  int* status;
-  int64_t most;  // keys that a table has room for
-  int32_t requests, tokens, G, HK, capacity, ctas, chain;
-};
+__device__ __forceinline__ int32_t tree_blocks(const TreeParams& p, const TreeEntry& e) {
+  return static_cast<int32_t>((static_cast<int64_t>(e.fresh) * p.G + 255) / 256);
+}
 
-__global__ void __launch_bounds__(kTreePlanThreads) tree_plan_kernel(const TreePlanParams p) {
-  __shared__ int32_t before[kTreePlanShared];
-  __shared__ int64_t warp_e[kTreePlanThreads / 32], warp_u[kTreePlanThreads / 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  grid_launch_dependents();
-  int64_t e_base = 0, u_base = 0;
-  for (int r0 = 0; r0 < p.requests; r0 += kTreePlanThreads) {
-    const int r = r0 + static_cast<int>(threadIdx.x);
-    TreeEntry t = {};
-    int32_t blocks = 0;
-    auto tiles_of = [&](int32_t block) {
-      int32_t end = t.len;
-      if (p.chain) {  // the block's last token sees no newer one
-        const int64_t last = min(static_cast<int64_t>(t.fresh) * p.G, (block + 1) * static_cast<int64_t>(256)) - 1;
-        end = min(end, t.ctx + static_cast<int32_t>(last / p.G) + 1);
+// Tiles of keys that a block's rows see some of; without a mask its last token
+// sees no newer one.
+__device__ __forceinline__ int32_t tree_tiles(const TreeParams& p, const TreeEntry& e, int32_t block) {
+  int32_t end = e.len;
+  if (p.mask == nullptr) {
+    const int32_t rows = min(e.fresh * p.G, (block + 1) * 256);
+    end = min(end, e.ctx + (rows - 1) / p.G + 1);
+  }
+  return max((end + 127) / 128, 1);
+}
+
+// The share of this CTA. All threads of the block take part; `sums` is scratch in
+// shared memory for two int64 per warp, and `out` shared too.
+template <uint32_t kThreads>
+__device__ __forceinline__ void find_share(const TreeParams& p, int64_t* sums, ShareStart* out) {
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr uint32_t kWarps = kThreads / 32;
+  auto tiles_of = [&](int32_t r, bool report) {
+    if (r >= p.requests) return static_cast<int64_t>(0);
+    const TreeEntry e = tree_request(p, r, report);
+    const int32_t blocks = tree_blocks(p, e);
+    int64_t n = 0;
+    for (int32_t b = 0; b < blocks; ++b) n += tree_tiles(p, e, b);
+    return n;
+  };
+  int64_t first = 0, sum = 0;  // this thread's first request, and all of them
+  for (int32_t r0 = 0; r0 < p.requests; r0 += static_cast<int32_t>(kThreads)) {
+    const int64_t n = tiles_of(r0 + static_cast<int32_t>(threadIdx.x), blockIdx.x == 0);
+    if (r0 == 0) first = n;
+    sum += n;
+  }
+  int64_t scan = first;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t up = __shfl_up_sync(0xffffffffu, scan, d);
+    if (lane >= static_cast<uint32_t>(d)) scan += up;
+  }
+  if (lane == 31u) sums[warp] = scan;
+  if (lane == 0u) sums[kWarps + warp] = sum;
+  __syncthreads();
+  int64_t total = 0, base = 0, upto = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < kWarps; ++i) {
+    total += sums[kWarps + i];
+    if (i < warp) base += sums[i];
+    upto += sums[i];
+  }
+  const int64_t units = total * p.HK;
+  const int64_t ctas = min(units, static_cast<int64_t>(gridDim.x));
+  const int64_t u = ctas > 0 ? units * blockIdx.x / ctas : 0;
+  if (threadIdx.x == 0) out->units = units;
+  if (static_cast<int64_t>(blockIdx.x) >= ctas) return;
+  int64_t n = first, before = base + scan - first;  // tiles of this thread's request, and before it
+  for (int32_t r0 = 0;;) {
+    if (n > 0 && before * p.HK <= u && u < (before + n) * p.HK) {
+      const int32_t r = r0 + static_cast<int32_t>(threadIdx.x);
+      const TreeEntry e = tree_request(p, r, false);
+      int32_t b = 0, tiles = tree_tiles(p, e, 0);
+      while (u >= (before + tiles) * p.HK) {
+        before += tiles;
+        tiles = tree_tiles(p, e, ++b);
       }
-      return max((end + 127) / 128, 1);
-    };
-    int64_t e = 0, u = 0;
-    if (r < p.requests) {
-      const int32_t lo = p.cu[r], hi = p.cu[r + 1];
-      const int32_t len = p.lens[r];
-      t.request = r;
-      t.first = min(max(lo, 0), p.tokens);
-      t.fresh = min(max(hi, t.first), p.tokens) - t.first;
-      t.len = static_cast<int32_t>(min(static_cast<int64_t>(max(len, 0)), p.most));
-      t.ctx = t.len - t.fresh;
-      if (p.status != nullptr) {
-        if (lo < 0 || hi < lo || hi > p.tokens) atomicCAS(p.status, 0, B2G_STATUS_TOKENS);
-        if (len > p.most) atomicCAS(p.status, 0, B2G_STATUS_PAGE_TABLE);
-      }
-      blocks = static_cast<int32_t>((static_cast<int64_t>(t.fresh) * p.G + 255) / 256);
-      e = blocks;
-      for (int32_t b = 0; b < blocks; ++b) u += tiles_of(b);
+      const int64_t in = u - before * p.HK;
+      out->before = before * p.HK;
+      out->request = r;
+      out->block = b;
+      out->hk = static_cast<int32_t>(in / tiles);
+      out->tile = static_cast<int32_t>(in % tiles);
     }
-    int64_t es = e, us = u;
+    r0 += static_cast<int32_t>(kThreads);
+    // the same for all threads: whether the share begins in a later round of requests
+    if (r0 >= p.requests || u < upto * p.HK) break;
+    n = tiles_of(r0 + static_cast<int32_t>(threadIdx.x), false);
+    scan = n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int64_t ue = __shfl_up_sync(0xffffffffu, es, d), uu = __shfl_up_sync(0xffffffffu, us, d);
-      if (lane >= d) {
-        es += ue;
-        us += uu;
-      }
+      const int64_t up = __shfl_up_sync(0xffffffffu, scan, d);
+      if (lane >= static_cast<uint32_t>(d)) scan += up;
     }
     __syncthreads();
-    if (lane == 31) {
-      warp_e[warp] = es;
-      warp_u[warp] = us;
-    }
+    if (lane == 31u) sums[warp] = scan;
     __syncthreads();
-    int64_t e_sum = 0, u_sum = 0;
-    for (int w = 0; w < kTreePlanThreads / 32; ++w) {
-      if (w < warp) {
-        es += warp_e[w];
-        us += warp_u[w];
-      }
-      e_sum += warp_e[w];
-      u_sum += warp_u[w];
+    before = upto + scan - n;
+#pragma unroll
+    for (uint32_t i = 0; i < kWarps; ++i) {
+      if (i < warp) before += sums[i];
+      upto += sums[i];
     }
-    int64_t at = e_base + es - e, sum = u_base + us - u;
-    for (int32_t b = 0; b < blocks; ++b, ++at) {
-      t.block = b;
-      t.tiles = tiles_of(b);
-      t.before = static_cast<int32_t>(sum);
-      sum += t.tiles;
-      if (at < p.capacity) p.plan[at] = t;
-      if (at < kTreePlanShared) before[at] = t.before;
-    }
-    e_base += e_sum;
-    u_base += u_sum;
-  }
-  __syncthreads();
-  // offsets that decrease can ask for more blocks than there is room for
-  const int32_t entries = static_cast<int32_t>(min(e_base, static_cast<int64_t>(p.capacity)));
-  if (entries < e_base) u_base = p.plan[entries - 1].before + p.plan[entries - 1].tiles;
-  const int64_t units = u_base * p.HK;
-  if (threadIdx.x == 0) {
-    p.meta->entries = entries;
-    p.meta->units = units;
-  }
-  const int64_t ctas = min(units, static_cast<int64_t>(p.ctas));
-  for (int c = threadIdx.x; c < ctas; c += kTreePlanThreads) {
-    const int64_t u = units * c / ctas;
-    int lo = 0, hi = entries - 1;  // the last entry that begins at or before u
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      const int64_t b = mid < kTreePlanShared ? before[mid] : p.plan[mid].before;
-      if (b * p.HK <= u) lo = mid;
-      else hi = mid - 1;
-    }
-    const int64_t in = u - static_cast<int64_t>(p.plan[lo].before) * p.HK;
-    const int32_t tiles = p.plan[lo].tiles;
-    p.start[c] = make_int4(lo, static_cast<int32_t>(in / tiles), static_cast<int32_t>(in % tiles), 0);
   }
 }
 
@@ -234,47 +235,80 @@ __global__ void __launch_bounds__(kTreePlanThreads) tree_plan_kernel(const TreeP
 // The part of one (block, key/value head) that lies in this CTA's share.
 struct Segment {
   TreeEntry e;
-  int32_t entry, hk;
+  int64_t unit0;    // the block and head's first unit
+  int32_t hk;
   int32_t j0, j1;   // tiles
   int32_t row0, rows;
   bool two;         // above 128 rows: a row tile per warpgroup
   uint32_t slots;   // warpgroups with tiles to visit
 };
 
-// Walks a share: the segments of `left` units from (entry, hk, tile).
+// Walks a share: the segments of its `left` units.
 struct SegmentWalk {
-  int32_t entry, hk, tile;
-  int64_t left;
+  TreeEntry e;
+  int64_t left, before;  // before: units before the block
+  int32_t hk, tile;
+
+  __device__ __forceinline__ void begin(const TreeParams& p, const ShareStart& s, int64_t units_here) {
+    left = units_here;
+    before = s.before;
+    hk = s.hk;
+    tile = s.tile;
+    if (left > 0) {
+      e = tree_request(p, s.request, false);
+      e.block = s.block;
+      e.tiles = tree_tiles(p, e, s.block);
+    }
+  }
 
   __device__ __forceinline__ bool next(const TreeParams& p, Segment& s) {
     if (left <= 0) return false;
-    const int4* src = reinterpret_cast<const int4*>(p.plan + entry);
-    const int4 a = src[0], b = src[1];
-    s.e.request = a.x;
-    s.e.block = a.y;
-    s.e.tiles = a.z;
-    s.e.before = a.w;
-    s.e.ctx = b.x;
-    s.e.fresh = b.y;
-    s.e.first = b.z;
-    s.e.len = b.w;
-    s.entry = entry;
+    if (hk == p.HK) {  // the next block, of this request or of the next that has new tokens
+      before += static_cast<int64_t>(e.tiles) * p.HK;
+      hk = 0;
+      if (e.block + 1 < tree_blocks(p, e)) {
+        ++e.block;
+      } else {
+        do e = tree_request(p, e.request + 1, false);
+        while (e.fresh == 0);
+      }
+      e.tiles = tree_tiles(p, e, e.block);
+    }
+    s.e = e;
     s.hk = hk;
+    s.unit0 = before + static_cast<int64_t>(hk) * e.tiles;
     s.j0 = tile;
-    s.j1 = static_cast<int32_t>(min(static_cast<int64_t>(s.e.tiles), tile + left));
+    s.j1 = static_cast<int32_t>(min(static_cast<int64_t>(e.tiles), tile + left));
     left -= s.j1 - s.j0;
-    s.row0 = s.e.block * 256;
-    s.rows = min(256, s.e.fresh * p.G - s.row0);
+    s.row0 = e.block * 256;
+    s.rows = min(256, e.fresh * p.G - s.row0);
     s.two = s.rows > 128;
     s.slots = s.two || s.j1 - s.j0 > 1 ? 2u : 1u;
     tile = 0;
-    if (++hk == p.HK) {
-      hk = 0;
-      ++entry;
-    }
+    ++hk;
     return true;
   }
 };
+
+// The CTA whose share holds unit u, of `ctas` equal shares of `units`.
+__device__ __forceinline__ int32_t share_of(int64_t u, int64_t units, int32_t ctas) {
+  return static_cast<int32_t>(((u + 1) * ctas - 1) / units);
+}
+
+// What the join of a block that lies in several shares needs of it.
+struct OpenBlock {
+  int32_t owner;  // the CTA whose share has its first tile (-1: none)
+  int32_t parts;  // shares
+  int32_t first, hk, row0, rows;
+};
+
+// The place of tile j's K and V among a segment's loads (n tiles).
+__device__ __forceinline__ uint32_t k_order(bool two, int32_t j) {
+  return static_cast<uint32_t>(two || j == 0 ? 2 * j : 2 * j - 1);
+}
+__device__ __forceinline__ uint32_t v_order(bool two, int32_t j, int32_t n) {
+  return static_cast<uint32_t>(two || j + 1 == n ? 2 * j + 1 : 2 * j + 2);
+}
 
 // Bits of the 32 keys from kb on that new token i of the segment's request sees.
 __device__ __forceinline__ uint32_t seen_bits(const TreeParams& p, const TreeEntry& e, int32_t i,
@@ -479,24 +513,19 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
     tmem_alloc<1>(smem_u32(tmem_slot), 512);
     tmem_relinquish<1>();
   }
+  ShareStart* start = reinterpret_cast<ShareStart*>(smem + TP::kMlOff + 512);
+  find_share<TP::kThreads>(p, reinterpret_cast<int64_t*>(smem + TP::kMlOff), start);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-  grid_dependency_wait();  // the plan is complete
-
-  const int64_t units = p.meta->units;
+  const ShareStart share = *start;
+  const int64_t units = share.units;
   const int32_t ctas =
       static_cast<int32_t>(min(units, static_cast<int64_t>(gridDim.x)));
   const int32_t me = static_cast<int32_t>(blockIdx.x);
-  SegmentWalk walk = {0, 0, 0, 0};
-  if (me < ctas) {
-    const int4 st = p.start[me];
-    walk.entry = st.x;
-    walk.hk = st.y;
-    walk.tile = st.z;
-    walk.left = units * (me + 1) / ctas - units * me / ctas;
-  }
+  SegmentWalk walk;
+  walk.begin(p, share, me < ctas ? units * (me + 1) / ctas - units * me / ctas : 0);
   Segment w;
 
   if (warp == 0) {
@@ -511,35 +540,43 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
     bool alive = true;
     while (alive && walk.next(p, w)) {
       const int32_t* table = p.tables + w.e.request * p.table_stride;
-      // this lane's page of tile j; num_pages, past the end, where there is none
+      // this lane's page of tile j, as the table has it; -2 for keys past the end
       auto page_of = [&](int32_t j) {
         const int32_t key = j * 128 + static_cast<int32_t>(box) * box_rows;
-        if (!issues || key >= w.e.len) return p.num_pages;
-        const int32_t page = table[key / p.page_size];
-        if (page >= 0 && page < p.num_pages) return page;
-        fmha_report(p, B2G_STATUS_PAGE_TABLE);
-        return p.num_pages;
+        return issues && key < w.e.len ? table[key / p.page_size] : -2;
       };
-      int32_t page = page_of(w.j0);
-      for (int32_t j = w.j0; alive && j < w.j1; ++j) {
-        const int32_t next = j + 1 < w.j1 ? page_of(j + 1) : 0;
-        const int32_t slot_row = p.page_size > 128 ? (j * 128) % p.page_size : 0;
-        for (uint32_t kv = 0; kv < 2; ++kv, ++ld) {
-          const uint32_t s = ld % NS;
-          if (!__all_sync(0xffffffffu, fmha_wait(empty(s), ((ld / NS) & 1u) ^ 1u, abort_flag, p,
-                                                 B2G_SITE_EMPTY))) {
-            alive = false;
-            break;
-          }
-          if (lane == 0) mbar_arrive_expect_tx(full(s), TP::kTile);
-          __syncwarp();
-          if (issues)
-            tma_load_4d(sbase + TP::kRingOff + s * TP::kTile + slab * kSlabBytes +
-                            box * static_cast<uint32_t>(box_rows) * 128u,
-                        kv == 0 ? &p.tmK : &p.tmV, full(s), static_cast<int32_t>(slab) * 64,
-                        slot_row, w.hk, page);
+      auto load = [&](const CUtensorMap* map, int32_t j, int32_t page) {
+        const uint32_t s = ld % NS;
+        if (!__all_sync(0xffffffffu, fmha_wait(empty(s), ((ld / NS) & 1u) ^ 1u, abort_flag, p,
+                                               B2G_SITE_EMPTY))) {
+          alive = false;
+          return;
         }
-        page = next;
+        if (lane == 0) mbar_arrive_expect_tx(full(s), TP::kTile);
+        __syncwarp();
+        if (issues) {
+          if (page < 0 || page >= p.num_pages) {  // past the last page: the box reads zeros
+            if (page != -2) fmha_report(p, B2G_STATUS_PAGE_TABLE);
+            page = p.num_pages;
+          }
+          tma_load_4d(sbase + TP::kRingOff + s * TP::kTile + slab * kSlabBytes +
+                          box * static_cast<uint32_t>(box_rows) * 128u,
+                      map, full(s), static_cast<int32_t>(slab) * 64,
+                      p.page_size > 128 ? (j * 128) % p.page_size : 0, w.hk, page);
+        }
+        ++ld;
+      };
+      // In the order in which the products take them: with two row tiles K and V of
+      // a tile, else K a tile ahead of V. Pages are read two tiles ahead.
+      int32_t page = page_of(w.j0), page1 = w.j0 + 1 < w.j1 ? page_of(w.j0 + 1) : -2;
+      load(&p.tmK, w.j0, page);
+      for (int32_t j = w.j0; alive && j < w.j1; ++j) {
+        const int32_t page2 = j + 2 < w.j1 ? page_of(j + 2) : -2;
+        if (w.two) load(&p.tmV, j, page);
+        if (alive && j + 1 < w.j1) load(&p.tmK, j + 1, page1);
+        if (alive && !w.two) load(&p.tmV, j, page);
+        page = page1;
+        page1 = page2;
       }
     }
     // every load issued lands before the CTA can exit
@@ -559,13 +596,13 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
       bool alive = true;
       while (alive && walk.next(p, w)) {
         const int32_t n = w.j1 - w.j0;
+        auto k_load = [&](int32_t j) { return base + k_order(w.two, j); };
         auto ready = [&](uint32_t load) {
           return fmha_wait(full(load % NS), (load / NS) & 1u, abort_flag, p, B2G_SITE_FULL);
         };
         // S = Q K^T of step j for warpgroup t
         auto issue_s = [&](uint32_t t, int32_t j) {
-          const uint32_t k_base =
-              sbase + TP::kRingOff + ((base + 2u * static_cast<uint32_t>(j)) % NS) * TP::kTile;
+          const uint32_t k_base = sbase + TP::kRingOff + (k_load(j) % NS) * TP::kTile;
           const uint32_t q_base = sbase + TP::kQOff + (w.two ? t * TP::kTile : 0u);
 #pragma unroll
           for (uint32_t kk = 0; kk < D / 16; ++kk) {
@@ -578,14 +615,14 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
           last_par = steps[t] & 1u;
           // the tile of K is free after its last product, Q after the block's
           if (!w.two || t == 1u) {
-            tc_commit<1>(empty((base + 2u * static_cast<uint32_t>(j)) % NS));
+            tc_commit<1>(empty(k_load(j) % NS));
             if (j + 1 == n) tc_commit<1>(q_empty);
           }
         };
         if (!fmha_wait(q_full, ic & 1u, abort_flag, p, B2G_SITE_FULL)) break;
         for (uint32_t t = 0; t < w.slots; ++t) {
           const int32_t j = w.two ? 0 : static_cast<int32_t>(t);
-          if (!ready(base + 2u * static_cast<uint32_t>(j))) {
+          if (!ready(k_load(j))) {
             alive = false;
             break;
           }
@@ -593,7 +630,7 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
           issue_s(t, j);
         }
         for (int32_t j = 0; alive && j < n; ++j) {
-          const uint32_t v_load = base + 2u * static_cast<uint32_t>(j) + 1u;
+          const uint32_t v_load = base + v_order(w.two, j, n);
           if (!ready(v_load)) {
             alive = false;
             break;
@@ -633,7 +670,7 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
               ++titems[t];
               continue;
             }
-            if (!ready(base + 2u * static_cast<uint32_t>(next))) {
+            if (!ready(k_load(next))) {
               alive = false;
               break;
             }
@@ -677,7 +714,7 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
       return wait_all(join, joins++, B2G_SITE_FLAG);
     };
     // blocks of this share that other shares hold parts of: the first and the last
-    int32_t open_entry[2] = {-1, -1}, open_hk[2] = {0, 0};
+    OpenBlock open_first = {-1}, open_last = {-1};
 
     while (alive && walk.next(p, w)) {
       const bool whole = w.j0 == 0 && w.j1 == w.e.tiles;
@@ -726,7 +763,7 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
         // Above one copy a row's weights are zero outside its columns, so every tile
         // is looked through; above 128 rows the first warpgroup does it for both.
         if ((masked || copies > 1u) && !(w.two && t == 1u)) {
-          const uint32_t load = base + 2u * static_cast<uint32_t>(j) + 1u;
+          const uint32_t load = base + v_order(w.two, j, n);
           if (!wait_all(full(load % NS), load / NS, B2G_SITE_FULL)) break;
           const bool mine = clear_odd_values<D, kBF16>(
               sbase + TP::kRingOff + (load % NS) * TP::kTile + row * 128u, lane);
@@ -766,7 +803,8 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
       }
       // where the rows go: O, or this share's unfinished rows
       const int32_t part_id = 2 * me + (w.j0 == 0 ? 1 : 0);
-      float* part = p.part + static_cast<int64_t>(part_id) * p.part_rows * D;
+      float4* part = reinterpret_cast<float4*>(p.part) +
+                     static_cast<int64_t>(part_id) * p.part_rows * (D / 4);
       float2* part_ml = p.part_ml + static_cast<int64_t>(part_id) * p.part_rows;
       constexpr float kLn2 = 0.693147180559945309f;
       auto store_sums = [&](float m, float l) {  // of this thread's row
@@ -805,12 +843,14 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
             }
             if (any_odd) add_odd_cache_values<D, T>(p, w, tok, 0, D, dst);
           } else {
-            float* dst = part + static_cast<int64_t>(brow) * D;
 #pragma unroll
             for (int v = 0; v < D / 4; ++v)
-              reinterpret_cast<uint4*>(dst)[v] =
-                  make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
-            if (any_odd) add_odd_cache_values<D, T>(p, w, tok, 0, D, dst);
+              part[v * p.part_rows + brow] =
+                  make_float4(__uint_as_float(o[4 * v]), __uint_as_float(o[4 * v + 1]),
+                              __uint_as_float(o[4 * v + 2]), __uint_as_float(o[4 * v + 3]));
+            if (any_odd)
+              for (int v = 0; v < D / 4; ++v)
+                add_odd_cache_values<D, T>(p, w, tok, 4 * v, 4, &part[v * p.part_rows + brow].x);
           }
         }
       } else {
@@ -821,56 +861,76 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
         const volatile uint32_t* ow = odd_words + (ic & 1u) * 8u;
         bool any_odd = (ow[0] | ow[1] | ow[2] | ow[3]) != 0u;
         if (w.slots == 2u) any_odd |= (ow[4] | ow[5] | ow[6] | ow[7]) != 0u;
+        const uint32_t parts = w.slots * copies;  // at most eight
+        // warp of part c that holds this row, or row r
+        auto warp_of = [&](uint32_t c, uint32_t r) {
+          return (c / copies) * 4u + (c % copies) * per + (r >> 5);
+        };
         float m_tot = -INFINITY, l_tot = 0.0f;
-        for (uint32_t c = 0; c < w.slots * copies; ++c)
-          m_tot = fmaxf(m_tot, ml[((c / copies) * 4u + (c % copies) * per + quarter % per) * 32u + lane].x);
-        for (uint32_t c = 0; c < w.slots * copies; ++c) {
-          const float2 x = ml[((c / copies) * 4u + (c % copies) * per + quarter % per) * 32u + lane];
-          if (m_tot > -INFINITY) l_tot = fmaf(x.y, fast_exp2(x.x - m_tot), l_tot);
+        {
+          float2 x[8];
+#pragma unroll
+          for (uint32_t c = 0; c < 8; ++c)
+            x[c] = c < parts ? ml[warp_of(c, static_cast<uint32_t>(lrow)) * 32u + lane]
+                             : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+          for (uint32_t c = 0; c < 8; ++c) m_tot = fmaxf(m_tot, x[c].x);
+          if (m_tot > -INFINITY)
+#pragma unroll
+            for (uint32_t c = 0; c < 8; ++c) l_tot = fmaf(x[c].y, fast_exp2(x[c].x - m_tot), l_tot);
         }
         float scale = m_tot > -INFINITY ? fast_exp2(m_run - m_tot) : 0.0f;
         if (whole) scale = l_tot == 0.0f ? 0.0f : scale / l_tot;
         if (t == 0u && copy == 0u && real) store_sums(m_tot, l_tot);
-        constexpr uint32_t JC = TP::kJoinCols, JV = JC / 4;  // columns, float4s of a row and round
+        // A round takes 32 columns, or as many as the buffer holds of fewer rows: it
+        // is [8 warps][row][columns], the float4s of a row permuted so that eight
+        // rows at once spread over the banks.
+        const uint32_t wrows = w.rows <= 8 ? 8u : w.rows <= 16 ? 16u : 32u;  // rows of a warp
+        const uint32_t cols = min(static_cast<uint32_t>(D), TP::kTile / (8u * 4u) / wrows);
+        const uint32_t vecs = cols / 4u;  // a power of two
         const uint32_t buf = sbase + TP::kJoinOff;
-        // float4 v of row r: the rows of eight lanes spread over the banks
         auto at = [&](uint32_t wq, uint32_t r, uint32_t v) {
-          return buf + ((wq * 32u + r) * JV + (v ^ (r & (JV - 1u)))) * 16u;
+          return buf + ((wq * wrows + r) * vecs + (v ^ (r & (vecs - 1u) & 7u))) * 16u;
         };
-        for (uint32_t d = 0; d < static_cast<uint32_t>(D); d += JC) {
+        for (uint32_t d = 0; d < static_cast<uint32_t>(D); d += cols) {
           if (active) {
-            uint32_t o[JC];
-            if constexpr (JC == 32) tmem_ld_32x32b_x32(o_col + d, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
-            else tmem_ld_32x32b_x16(o_col + d, *reinterpret_cast<uint32_t(*)[16]>(&o[0]));
-            tmem_wait_ld();
-            if (d + JC == static_cast<uint32_t>(D)) {
+#pragma unroll 1
+            for (uint32_t d2 = 0; d2 < cols; d2 += 16u) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(o_col + d + d2, o);
+              tmem_wait_ld();
+              if (real) {
+#pragma unroll
+                for (uint32_t v = 0; v < 4; ++v) {
+                  uint32_t x[4];
+#pragma unroll
+                  for (uint32_t i = 0; i < 4; ++i)
+                    x[i] = __float_as_uint(__uint_as_float(o[4 * v + i]) * scale);
+                  st_shared_v4(at(t * 4u + quarter, lane, d2 / 4u + v), x);
+                }
+              }
+            }
+            if (d + cols == static_cast<uint32_t>(D)) {
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(o_free(t));
             }
-            if (real) {
-#pragma unroll
-              for (uint32_t v = 0; v < JV; ++v) {
-                uint32_t x[4];
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i)
-                  x[i] = __float_as_uint(__uint_as_float(o[4 * v + i]) * scale);
-                st_shared_v4(at(t * 4u + quarter, lane, v), x);
-              }
-            }
           }
           if (!meet()) break;
           // four columns of one row to a thread
-          for (uint32_t i = threadIdx.x - 64u; i < static_cast<uint32_t>(w.rows) * JV; i += 256u) {
-            const uint32_t r = i / JV, v = i % JV;
+          for (uint32_t i = threadIdx.x - 64u; i < static_cast<uint32_t>(w.rows) * vecs; i += 256u) {
+            const uint32_t r = i / vecs, v = i % vecs;
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (uint32_t c = 0; c < w.slots * copies; ++c) {
-              uint32_t x[4];
-              ld_shared_v4(at((c / copies) * 4u + (c % copies) * per + (r >> 5), r & 31u, v), x);
-              sum.x += __uint_as_float(x[0]);
-              sum.y += __uint_as_float(x[1]);
-              sum.z += __uint_as_float(x[2]);
-              sum.w += __uint_as_float(x[3]);
+#pragma unroll
+            for (uint32_t c = 0; c < 8; ++c) {
+              if (c < parts) {
+                uint32_t x[4];
+                ld_shared_v4(at(warp_of(c, r), r & 31u, v), x);
+                sum.x += __uint_as_float(x[0]);
+                sum.y += __uint_as_float(x[1]);
+                sum.z += __uint_as_float(x[2]);
+                sum.w += __uint_as_float(x[3]);
+              }
             }
             const int32_t g = w.row0 + static_cast<int32_t>(r), tk = g / p.G;
             const int32_t col = static_cast<int32_t>(d + 4u * v);
@@ -881,9 +941,9 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
                   make_uint2(pack2<kBF16>(sum.x, sum.y), pack2<kBF16>(sum.z, sum.w));
               if (any_odd) add_odd_cache_values<D, T>(p, w, tk, col, 4, dst);
             } else {
-              float* dst = part + static_cast<int64_t>(r) * D + col;
-              *reinterpret_cast<float4*>(dst) = sum;
-              if (any_odd) add_odd_cache_values<D, T>(p, w, tk, col, 4, dst);
+              float4* dst = part + (col / 4) * p.part_rows + r;
+              *dst = sum;
+              if (any_odd) add_odd_cache_values<D, T>(p, w, tk, col, 4, &dst->x);
             }
           }
           if (!meet()) break;  // the buffer is free again
@@ -891,36 +951,38 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
         if (!alive) break;
       }
       if (!whole) {
-        // publish: every warp's rows are written, then the owner's count goes up
-        if (!meet()) break;
-        const int64_t u0 = static_cast<int64_t>(w.e.before) * p.HK + static_cast<int64_t>(w.hk) * w.e.tiles;
-        if (warp == 2u && lane == 0) {
-          __threadfence();
-          atomicAdd(&p.counters[2 * share_of(u0, units, ctas)], 1u);
-        }
-        const int slot = w.j1 == w.e.tiles ? 0 : 1;
-        open_entry[slot] = w.entry;
-        open_hk[slot] = w.hk;
+        OpenBlock b;
+        b.owner = share_of(w.unit0, units, ctas);
+        b.parts = share_of(w.unit0 + w.e.tiles - 1, units, ctas) - b.owner + 1;
+        b.first = w.e.first;
+        b.hk = w.hk;
+        b.row0 = w.row0;
+        b.rows = w.rows;
+        (w.j1 == w.e.tiles ? open_first : open_last) = b;
       }
       base += 2u * static_cast<uint32_t>(n);
       ++ic;
     }
 
-    // The blocks that this share had a part of: when every part is published, each
-    // of the CTAs joins its slice of the block's values, in the order of the shares.
+    // The blocks that this share had a part of: this CTA's parts are published, and
+    // when all of a block's are, each of its CTAs joins a slice of the block's
+    // values, in the order of the shares.
+    if (alive && (open_first.owner >= 0 || open_last.owner >= 0) && meet()) {
+      const int32_t owner = lane == 0 ? open_first.owner : open_last.owner;
+      if (warp == 2u && lane < 2u && owner >= 0) {
+        __threadfence();
+        atomicAdd(&p.counters[2 * owner], 1u);
+      }
+    }
 #pragma unroll 1
     for (int slot = 0; alive && slot < 2; ++slot) {
-      if (open_entry[slot] < 0) continue;
-      const TreeEntry e = p.plan[open_entry[slot]];
-      const int32_t hk = open_hk[slot];
-      const int64_t u0 = static_cast<int64_t>(e.before) * p.HK + static_cast<int64_t>(hk) * e.tiles;
-      const int32_t owner = share_of(u0, units, ctas);
-      const int32_t parts = share_of(u0 + e.tiles - 1, units, ctas) - owner + 1;
-      uint32_t* count = p.counters + 2 * owner;
+      const OpenBlock b = slot == 0 ? open_first : open_last;
+      if (b.owner < 0) continue;
+      uint32_t* count = p.counters + 2 * b.owner;
       bool there = true;
       if (lane == 0) {
         const uint64_t t0 = globaltimer_ns();
-        while (ld_acquire_gpu(count) < static_cast<uint32_t>(parts)) {
+        while (ld_acquire_gpu(count) < static_cast<uint32_t>(b.parts)) {
           if (*abort_flag != 0u || globaltimer_ns() - t0 > p.timeout_ns) {
             fmha_report(p, B2G_STATUS_TIMEOUT | B2G_SITE_FLAG);
             *abort_flag = 1u;
@@ -933,47 +995,61 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
         alive = false;
         break;
       }
-      const int32_t row0 = e.block * 256, rows = min(256, e.fresh * p.G - row0);
-      constexpr int32_t kV = D / 4;
-      const int64_t all = static_cast<int64_t>(rows) * kV;
-      const int32_t k = me - owner;
-      const int64_t stop = all * (k + 1) / parts;
-      for (int64_t i = all * k / parts + (threadIdx.x - 64u); i < stop; i += 256) {
-        const int32_t r = static_cast<int32_t>(i / kV), v = static_cast<int32_t>(i % kV);
-        auto id = [&](int32_t c) { return static_cast<int64_t>(c == 0 ? 2 * owner + 1 : 2 * (owner + c)); };
-        float m = -INFINITY;
-#pragma unroll 4
-        for (int32_t c = 0; c < parts; ++c) m = fmaxf(m, __ldcg(&p.part_ml[id(c) * p.part_rows + r]).x);
-        float l = 0.0f;
+      // a float4 of one row to a thread, neighbours in the row index
+      const int32_t k = me - b.owner;
+      const int64_t all = static_cast<int64_t>(b.rows) * (D / 4);
+      const int64_t stop = all * (k + 1) / b.parts;
+      for (int64_t i = all * k / b.parts + (threadIdx.x - 64u); i < stop; i += 256) {
+        const int32_t r = static_cast<int32_t>(i % b.rows), v = static_cast<int32_t>(i / b.rows);
+        float m = -INFINITY, l = 0.0f;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (m > -INFINITY) {
-#pragma unroll 4
-          for (int32_t c = 0; c < parts; ++c) {
-            const float2 x = __ldcg(&p.part_ml[id(c) * p.part_rows + r]);
-            const float4 o = __ldcg(reinterpret_cast<const float4*>(
-                p.part + (id(c) * p.part_rows + r) * D) + v);
-            const float f = fast_exp2(x.x - m);
-            l = fmaf(x.y, f, l);
-            sum.x = fmaf(o.x, f, sum.x);
-            sum.y = fmaf(o.y, f, sum.y);
-            sum.z = fmaf(o.z, f, sum.z);
-            sum.w = fmaf(o.w, f, sum.w);
+        for (int32_t c0 = 0; c0 < b.parts; c0 += kJoinBatch) {
+          float2 x[kJoinBatch];
+          float4 o[kJoinBatch];
+#pragma unroll
+          for (int32_t c = 0; c < kJoinBatch; ++c) {
+            x[c] = make_float2(-INFINITY, 0.0f);
+            o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (c0 + c < b.parts) {
+              const int64_t id = c0 + c == 0 ? 2 * b.owner + 1 : 2 * (b.owner + c0 + c);
+              x[c] = __ldcg(&p.part_ml[id * p.part_rows + r]);
+              o[c] = __ldcg(reinterpret_cast<const float4*>(p.part) +
+                            (id * (D / 4) + v) * p.part_rows + r);
+            }
+          }
+          float top = m;
+#pragma unroll
+          for (int32_t c = 0; c < kJoinBatch; ++c) top = fmaxf(top, x[c].x);
+          if (top == -INFINITY) continue;  // nothing seen so far
+          const float was = fast_exp2(m - top);
+          l *= was;
+          sum = make_float4(sum.x * was, sum.y * was, sum.z * was, sum.w * was);
+          m = top;
+#pragma unroll
+          for (int32_t c = 0; c < kJoinBatch; ++c) {
+            if (c0 + c >= b.parts) continue;
+            const float f = fast_exp2(x[c].x - m);
+            l = fmaf(x[c].y, f, l);
+            sum.x = fmaf(o[c].x, f, sum.x);
+            sum.y = fmaf(o[c].y, f, sum.y);
+            sum.z = fmaf(o[c].z, f, sum.z);
+            sum.w = fmaf(o[c].w, f, sum.w);
           }
         }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const int32_t g = row0 + r, tk = g / p.G, h = hk * p.G + g % p.G;
-        T* dst = static_cast<T*>(p.O) + static_cast<int64_t>(e.first + tk) * p.o_t + h * p.o_h + 4 * v;
+        const int32_t g = b.row0 + r, tk = b.first + g / p.G, h = b.hk * p.G + g % p.G;
+        T* dst = static_cast<T*>(p.O) + static_cast<int64_t>(tk) * p.o_t + h * p.o_h + 4 * v;
         *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<kBF16>(sum.x * inv, sum.y * inv),
                                                     pack2<kBF16>(sum.z * inv, sum.w * inv));
         if (v == 0 && p.lse != nullptr)
-          p.lse[static_cast<int64_t>(h) * p.tokens + e.first + tk] =
+          p.lse[static_cast<int64_t>(h) * p.tokens + tk] =
               l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.693147180559945309f;
       }
       // the last CTA to have read the parts leaves both counts at zero
       if (!meet()) break;
       if (warp == 2u && lane == 0) {
         __threadfence();
-        if (atomicAdd(&count[1], 1u) + 1u == static_cast<uint32_t>(parts)) {
+        if (atomicAdd(&count[1], 1u) + 1u == static_cast<uint32_t>(b.parts)) {
           count[0] = 0u;
           count[1] = 0u;
         }
@@ -993,20 +1069,15 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
 namespace {
 
 struct TreeWorkspace {
-  size_t meta, start, plan, part, part_ml, total;
-  int64_t capacity;  // row blocks
+  size_t part, part_ml, total;
   int32_t part_rows;
 };
 
-TreeWorkspace tree_workspace(int requests, int64_t tokens, int group, int head_dim, int sms) {
+TreeWorkspace tree_workspace(int64_t tokens, int group, int head_dim, int sms) {
   TreeWorkspace w;
   auto up = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
-  w.capacity = tokens * group / 256 + std::min<int64_t>(requests, tokens);
   w.part_rows = static_cast<int32_t>(std::min<int64_t>(256, tokens * group));
-  w.meta = workspace_flag_bytes(sms);
-  w.start = w.meta + 256;
-  w.plan = w.start + up(sizeof(int4) * static_cast<size_t>(sms));
-  w.part_ml = w.plan + up(sizeof(TreeEntry) * static_cast<size_t>(w.capacity));
+  w.part_ml = workspace_flag_bytes(sms);
   w.part = w.part_ml + up(sizeof(float2) * 2 * static_cast<size_t>(sms) * w.part_rows);
   w.total = w.part + sizeof(float) * 2 * static_cast<size_t>(sms) * w.part_rows * head_dim;
   return w;
@@ -1048,18 +1119,8 @@ int launch_tree(const TreeParams& prm, int sms, cudaStream_t stream) {
   }
   // one CTA per SM: the CTAs that share a block wait for one another, so all of
   // them have to be resident
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(sms), 1, 1);
-  cfg.blockDim = dim3(TP::kThreads, 1, 1);
-  cfg.dynamicSmemBytes = TP::kDynBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, prm);
-  if (e != cudaSuccess) cudaGetLastError();
+  kern<<<static_cast<unsigned>(sms), TP::kThreads, TP::kDynBytes, stream>>>(prm);
+  const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? B2G_OK : static_cast<int>(e);
 }
 
@@ -1072,7 +1133,7 @@ extern "C" size_t b2g_attention_tree_workspace_bytes(int requests, int64_t token
   const int sms = b2g::current_device_sms();
   if (sms <= 0 || requests < 0 || tokens < 0 || heads_k < 1 || heads_q < heads_k || head_dim < 1)
     return 0;
-  return b2g::tree_workspace(requests, tokens, heads_q / heads_k, head_dim, sms).total;
+  return b2g::tree_workspace(tokens, heads_q / heads_k, head_dim, sms).total;
 }
 
 extern "C" int b2g_attention_tree(const void* q, const void* k_cache, const void* v_cache, void* o,
@@ -1103,7 +1164,7 @@ extern "C" int b2g_attention_tree(const void* q, const void* k_cache, const void
     return B2G_EALIGN;
   const int sms = current_device_sms();
   if (sms <= 0) return B2G_ENODEVICE;
-  const TreeWorkspace wl = tree_workspace(requests, tokens, group, head_dim, sms);
+  const TreeWorkspace wl = tree_workspace(tokens, group, head_dim, sms);
   if (workspace == nullptr || workspace_bytes < wl.total) return B2G_EWORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return B2G_EALIGN;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -1113,21 +1174,6 @@ extern "C" int b2g_attention_tree(const void* q, const void* k_cache, const void
   if (!encode_cache(&prm.tmK, k_cache, dtype, head_dim, page_size, heads_k, num_pages, strides + 2) ||
       !encode_cache(&prm.tmV, v_cache, dtype, head_dim, page_size, heads_k, num_pages, strides + 5))
     return B2G_ETENSORMAP;
-  TreePlanParams pl;
-  pl.cu = cu_seqlens;
-  pl.lens = seq_lens;
-  pl.plan = reinterpret_cast<TreeEntry*>(ws + wl.plan);
-  pl.meta = reinterpret_cast<TreeMeta*>(ws + wl.meta);
-  pl.start = reinterpret_cast<int4*>(ws + wl.start);
-  pl.status = status;
-  pl.most = std::min<int64_t>(static_cast<int64_t>(max_pages) * page_size, INT_MAX - 256);
-  pl.requests = requests;
-  pl.tokens = static_cast<int32_t>(tokens);
-  pl.G = group;
-  pl.HK = heads_k;
-  pl.capacity = static_cast<int32_t>(wl.capacity);
-  pl.ctas = sms;
-  pl.chain = tree_mask == nullptr;
   prm.Q = q;
   prm.q_t = strides[0];
   prm.q_h = strides[1];
@@ -1144,9 +1190,11 @@ extern "C" int b2g_attention_tree(const void* q, const void* k_cache, const void
   prm.mask_words = mask_words;
   prm.lse = lse;
   prm.status = status;
-  prm.plan = pl.plan;
-  prm.meta = pl.meta;
-  prm.start = pl.start;
+  prm.cu = cu_seqlens;
+  prm.lens = seq_lens;
+  prm.requests = requests;
+  prm.most = static_cast<int32_t>(
+      std::min<int64_t>(static_cast<int64_t>(max_pages) * page_size, INT_MAX - 256));
   prm.part = reinterpret_cast<float*>(ws + wl.part);
   prm.part_ml = reinterpret_cast<float2*>(ws + wl.part_ml);
   prm.part_rows = wl.part_rows;
@@ -1160,9 +1208,6 @@ extern "C" int b2g_attention_tree(const void* q, const void* k_cache, const void
   prm.scale_log2 = sm_scale * 1.4426950408889634f;
   prm.timeout_ns = wait_timeout_ns();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  tree_plan_kernel<<<1, kTreePlanThreads, 0, s>>>(pl);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return static_cast<int>(e);
   const bool bf16 = dtype == B2G_DT_BF16;
   if (head_dim == 128)
     return bf16 ? launch_tree<128, true>(prm, sms, s) : launch_tree<128, false>(prm, sms, s);
