@@ -55,11 +55,11 @@ struct TreeEntry {
   int32_t len;              // keys
 };
 
-// Where a share begins: block `block` of request `request`, head, tile; `before`
-// units lie before the block.
+// Where a share begins: head and tile of `e`; `before` units lie before the block.
 struct ShareStart {
-  int64_t units, before;
-  int32_t request, block, hk, tile;
+  int64_t units, before, here;  // here: units of the share
+  TreeEntry e;
+  int32_t hk, tile;
 };
 
 struct alignas(64) TreeParams {
@@ -87,8 +87,6 @@ struct alignas(64) TreeParams {
   uint64_t timeout_ns;
 };
 
-constexpr int32_t kJoinBatch = 8;  // parts of a block that a thread reads at once
-
 template <int D>
 struct TreePlan {
   static constexpr uint32_t kSoftmaxWarps = 8;
@@ -101,8 +99,8 @@ struct TreePlan {
   static constexpr uint32_t kRingOff = 2 * kTile;
   static constexpr uint32_t kMlOff = kRingOff + kSlots * kTile;   // float2 [8 warps][32 rows]
   static constexpr uint32_t kBarOff = kMlOff + 8 * 32 * 8;
-  // q_full, q_empty, full[S], empty[S], s_full[2], p_full[2][2], o_done[2], o_free[2], join
-  static constexpr uint32_t kNumBars = 2 + 2 * kSlots + 11;
+  // q_full, q_empty, full[S], empty[S], s_full[2], p_full[2][2], o_done[2], o_free[2]
+  static constexpr uint32_t kNumBars = 2 + 2 * kSlots + 10;
   static constexpr uint32_t kMiscOff = kBarOff + kNumBars * 8;  // tmem slot, abort flag
   static constexpr uint32_t kOddOff = kMiscOff + 16;            // [2 blocks][8 warps]
   static constexpr uint32_t kBytes = kOddOff + 64;
@@ -149,6 +147,22 @@ __device__ __forceinline__ int32_t tree_tiles(const TreeParams& p, const TreeEnt
   return max((end + 127) / 128, 1);
 }
 
+// Units before CTA c's of `ctas` equal shares, and the CTA whose share holds unit
+// u. A 64-bit division takes several hundred cycles, so 32-bit ones where they do.
+__device__ __forceinline__ int64_t mul_div(int64_t a, int64_t b, int64_t d) {
+  const int64_t n = a * b;
+  if (((n | d) >> 32) == 0) return static_cast<uint32_t>(n) / static_cast<uint32_t>(d);
+  return n / d;
+}
+__device__ __forceinline__ int64_t share_begin(int64_t units, int32_t c, int32_t ctas) {
+  return mul_div(units, c, ctas);
+}
+__device__ __forceinline__ int32_t share_of(int64_t u, int64_t units, int32_t ctas) {
+  // the last c whose share begins at or before u: c < (u + 1) ctas / units
+  const int64_t n = (u + 1) * ctas - 1;
+  return static_cast<int32_t>(mul_div(n, 1, units));
+}
+
 // The share of this CTA. All threads of the block take part; `sums` is scratch in
 // shared memory for two int64 per warp, and `out` shared too.
 template <uint32_t kThreads>
@@ -189,25 +203,30 @@ __device__ __forceinline__ void find_share(const TreeParams& p, int64_t* sums, S
   }
   const int64_t units = total * p.HK;
   const int64_t ctas = min(units, static_cast<int64_t>(gridDim.x));
-  const int64_t u = ctas > 0 ? units * blockIdx.x / ctas : 0;
-  if (threadIdx.x == 0) out->units = units;
+  const int64_t u =
+      ctas > 0 ? share_begin(units, static_cast<int32_t>(blockIdx.x), static_cast<int32_t>(ctas)) : 0;
+  if (threadIdx.x == 0) {
+    out->units = units;
+    out->here = 0;
+  }
   if (static_cast<int64_t>(blockIdx.x) >= ctas) return;
   int64_t n = first, before = base + scan - first;  // tiles of this thread's request, and before it
   for (int32_t r0 = 0;;) {
     if (n > 0 && before * p.HK <= u && u < (before + n) * p.HK) {
       const int32_t r = r0 + static_cast<int32_t>(threadIdx.x);
-      const TreeEntry e = tree_request(p, r, false);
-      int32_t b = 0, tiles = tree_tiles(p, e, 0);
-      while (u >= (before + tiles) * p.HK) {
-        before += tiles;
-        tiles = tree_tiles(p, e, ++b);
+      TreeEntry e = tree_request(p, r, false);
+      e.tiles = tree_tiles(p, e, 0);
+      while (u >= (before + e.tiles) * p.HK) {
+        before += e.tiles;
+        e.tiles = tree_tiles(p, e, ++e.block);
       }
-      const int64_t in = u - before * p.HK;
+      const int64_t in = u - before * p.HK;  // less than tiles * HK
+      out->here = share_begin(units, static_cast<int32_t>(blockIdx.x) + 1,
+                              static_cast<int32_t>(ctas)) - u;
       out->before = before * p.HK;
-      out->request = r;
-      out->block = b;
-      out->hk = static_cast<int32_t>(in / tiles);
-      out->tile = static_cast<int32_t>(in % tiles);
+      out->e = e;
+      out->hk = static_cast<int32_t>(mul_div(in, 1, e.tiles));
+      out->tile = static_cast<int32_t>(in - static_cast<int64_t>(out->hk) * e.tiles);
     }
     r0 += static_cast<int32_t>(kThreads);
     // the same for all threads: whether the share begins in a later round of requests
@@ -249,16 +268,12 @@ struct SegmentWalk {
   int64_t left, before;  // before: units before the block
   int32_t hk, tile;
 
-  __device__ __forceinline__ void begin(const TreeParams& p, const ShareStart& s, int64_t units_here) {
-    left = units_here;
+  __device__ __forceinline__ void begin(const ShareStart& s) {
+    left = s.here;
     before = s.before;
+    e = s.e;
     hk = s.hk;
     tile = s.tile;
-    if (left > 0) {
-      e = tree_request(p, s.request, false);
-      e.block = s.block;
-      e.tiles = tree_tiles(p, e, s.block);
-    }
   }
 
   __device__ __forceinline__ bool next(const TreeParams& p, Segment& s) {
@@ -289,11 +304,6 @@ struct SegmentWalk {
     return true;
   }
 };
-
-// The CTA whose share holds unit u, of `ctas` equal shares of `units`.
-__device__ __forceinline__ int32_t share_of(int64_t u, int64_t units, int32_t ctas) {
-  return static_cast<int32_t>(((u + 1) * ctas - 1) / units);
-}
 
 // What the join of a block that lies in several shares needs of it.
 struct OpenBlock {
@@ -460,6 +470,78 @@ __device__ __forceinline__ void tree_softmax(uint32_t s_col, uint32_t o_col, uin
   m_run = m_new;
 }
 
+// Joins share k of a block: a lane to a row, E float4 columns by P parts at a time,
+// whose loads are all in flight together (with eight warps on the SM their latency
+// and that of the arithmetic between them is what bounds this, so what depends on
+// the row alone is done once). More than P parts go in rounds with a running
+// maximum. Indices past the end repeat the last one: every load is unconditional.
+template <int D, bool kBF16, int E, int P>
+__device__ __noinline__ void join_parts(const TreeParams& p, const OpenBlock& b, int32_t k,
+                                        int32_t warp8, int32_t lane) {
+  using T = typename std::conditional<kBF16, __nv_bfloat16, __half>::type;
+  constexpr int32_t kRuns = D / 4 / E;  // runs of E columns in a row
+  const int32_t all = (b.rows + 31) / 32 * kRuns;
+  const int32_t to = all * (k + 1) / b.parts;
+  const int32_t part_step = 2 * (D / 4) * p.part_rows;  // float4s between two CTAs' parts
+  for (int32_t u = all * k / b.parts + warp8; u < to; u += 8) {
+    const int32_t r0 = u / kRuns * 32 + lane, r = min(r0, b.rows - 1), v = u % kRuns * E;
+    // the owner's part lies one slot after the others'
+    const float2* ml = p.part_ml + 2 * b.owner * p.part_rows + r;
+    const float4* po = reinterpret_cast<const float4*>(p.part) + b.owner * part_step +
+                       v * p.part_rows + r;
+    float m = -INFINITY, l = 0.0f;
+    float4 sum[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int32_t c0 = 0; c0 < b.parts; c0 += P) {
+      float2 x[P];
+      float4 o[P][E];
+#pragma unroll
+      for (int c = 0; c < P; ++c) {
+        const int32_t part = min(c0 + c, b.parts - 1), first = part == 0 ? 1 : 0;
+        x[c] = __ldcg(ml + (2 * part + first) * p.part_rows);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          o[c][e] = __ldcg(po + part * part_step + (first * (D / 4) + e) * p.part_rows);
+      }
+      float top = m;
+#pragma unroll
+      for (int c = 0; c < P; ++c) top = fmaxf(top, x[c].x);
+      if (top == -INFINITY) continue;  // the row has seen nothing so far
+      const float was = fast_exp2(m - top);
+      m = top;
+      l *= was;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        sum[e] = make_float4(sum[e].x * was, sum[e].y * was, sum[e].z * was, sum[e].w * was);
+#pragma unroll
+      for (int c = 0; c < P; ++c) {
+        if (c0 + c >= b.parts) continue;
+        const float f = fast_exp2(x[c].x - top);
+        l = fmaf(x[c].y, f, l);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          sum[e].x = fmaf(o[c][e].x, f, sum[e].x);
+          sum[e].y = fmaf(o[c][e].y, f, sum[e].y);
+          sum[e].z = fmaf(o[c][e].z, f, sum[e].z);
+          sum[e].w = fmaf(o[c][e].w, f, sum[e].w);
+        }
+      }
+    }
+    if (r0 >= b.rows) continue;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int32_t g = b.row0 + r, t = g / p.G, h = b.hk * p.G + g - t * p.G;
+    T* dst = static_cast<T*>(p.O) + static_cast<int64_t>(b.first + t) * p.o_t + h * p.o_h + 4 * v;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      reinterpret_cast<uint2*>(dst)[e] = make_uint2(pack2<kBF16>(sum[e].x * inv, sum[e].y * inv),
+                                                    pack2<kBF16>(sum[e].z * inv, sum[e].w * inv));
+    if (v == 0 && p.lse != nullptr)
+      p.lse[static_cast<int64_t>(h) * p.tokens + b.first + t] =
+          l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.693147180559945309f;
+  }
+}
+
 template <int D, bool kBF16>
 __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
     tree_kernel(const __grid_constant__ TreeParams p) {
@@ -485,7 +567,6 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
   auto p_full = [&](uint32_t t, uint32_t half) { return bar1 + 8u * (2 + 2 * t + half); };
   auto o_done = [&](uint32_t t) { return bar1 + 8u * (6 + t); };
   auto o_free = [&](uint32_t t) { return bar1 + 8u * (8 + t); };
-  const uint32_t join = bar1 + 8u * 10;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + TP::kMiscOff);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + TP::kMiscOff + 4);
 
@@ -503,7 +584,6 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
       mbar_init(o_done(t), 1);
       mbar_init(o_free(t), 4);
     }
-    mbar_init(join, TP::kSoftmaxWarps);
     *abort_flag = 0u;
     fence_mbarrier_init();
     prefetch_tensormap(&p.tmK);
@@ -525,7 +605,7 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
       static_cast<int32_t>(min(units, static_cast<int64_t>(gridDim.x)));
   const int32_t me = static_cast<int32_t>(blockIdx.x);
   SegmentWalk walk;
-  walk.begin(p, share, me < ctas ? units * (me + 1) / ctas - units * me / ctas : 0);
+  walk.begin(share);
   Segment w;
 
   if (warp == 0) {
@@ -700,35 +780,31 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
     volatile uint32_t* odd_words = reinterpret_cast<volatile uint32_t*>(smem + TP::kOddOff);
     uint32_t step = 0, ti = 0;        // this warpgroup's tiles and segments
     uint32_t base = 0, ic = 0;        // ring loads before the segment, segments of the CTA
-    uint32_t joins = 0;               // uses of the join barrier
     bool alive = true;
+    // The eight warps meet at a hardware barrier, which has no limit of its own: so a
+    // warp whose wait ran out does not leave, but goes on without waiting (its results
+    // no longer count, the status says so) and reaches every meeting like the others.
     auto wait_all = [&](uint32_t bar, uint32_t parity, int site) {
-      if (__all_sync(0xffffffffu, fmha_wait(bar, parity & 1u, abort_flag, p, site)) == 0)
+      if (alive && __all_sync(0xffffffffu, fmha_wait(bar, parity & 1u, abort_flag, p, site)) == 0)
         alive = false;
-      return alive;
     };
-    // all eight warps meet
-    auto meet = [&]() {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(join);
-      return wait_all(join, joins++, B2G_SITE_FLAG);
-    };
+    auto meet = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
     // blocks of this share that other shares hold parts of: the first and the last
     OpenBlock open_first = {-1}, open_last = {-1};
 
-    while (alive && walk.next(p, w)) {
+    while (walk.next(p, w)) {
       const bool whole = w.j0 == 0 && w.j1 == w.e.tiles;
-      const uint32_t copies = w.two || w.rows > 64 ? 1u : w.rows > 32 ? 2u : 4u;
-      const uint32_t per = 4u / copies;                  // warps of a copy
-      const uint32_t copy = quarter / per;
-      const int32_t lrow = static_cast<int32_t>((quarter % per) * 32u + lane);  // row in the tile
+      const uint32_t lc = w.two || w.rows > 64 ? 0u : w.rows > 32 ? 1u : 2u;
+      const uint32_t copies = 1u << lc, per = 4u >> lc;  // copies of the rows, warps of a copy
+      const uint32_t copy = quarter >> (2u - lc);
+      const int32_t lrow = static_cast<int32_t>((quarter & (per - 1u)) * 32u + lane);  // row in the tile
       const int32_t brow = lrow + (w.two ? static_cast<int32_t>(t) * 128 : 0);  // row in the block
       const bool real = brow < w.rows;
       const int32_t grow = w.row0 + brow;                // row of the (request, head)
-      const int32_t tok = grow / p.G, head = w.hk * p.G + grow % p.G;
+      const int32_t tok = grow / p.G, head = w.hk * p.G + grow - tok * p.G;
 
       // Q into shared memory: with one row tile each warpgroup copies half of every row
-      if (ic > 0 && !wait_all(q_empty, ic - 1u, B2G_SITE_EMPTY)) break;
+      if (ic > 0) wait_all(q_empty, ic - 1u, B2G_SITE_EMPTY);
       {
         constexpr uint32_t kVecs = static_cast<uint32_t>(D) / 8;  // 16-byte pieces of a row
         const uint32_t v0 = w.two ? 0u : t * (kVecs / 2), v1 = w.two ? kVecs : v0 + kVecs / 2;
@@ -736,12 +812,13 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
             static_cast<const T*>(p.Q) + (w.e.first + static_cast<int64_t>(real ? tok : 0)) * p.q_t +
             (real ? head : 0) * p.q_h);
         const uint32_t dst = sbase + TP::kQOff + (w.two ? t * TP::kTile : 0u) + row * 128u;
-        for (uint32_t v = v0; v < v1; v += 4) {
-          uint4 x[4];
+        constexpr uint32_t kBatch = kVecs / 2;
+        for (uint32_t v = v0; v < v1; v += kBatch) {
+          uint4 x[kBatch];
 #pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) x[i] = real ? src[v + i] : make_uint4(0, 0, 0, 0);
+          for (uint32_t i = 0; i < kBatch; ++i) x[i] = real ? src[v + i] : make_uint4(0, 0, 0, 0);
 #pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) {
+          for (uint32_t i = 0; i < kBatch; ++i) {
             // 128-byte swizzle: 16-byte piece c of row r sits at piece c ^ (r % 8)
             const uint32_t a = dst + ((v + i) >> 3) * kSlabBytes + ((((v + i) & 7u) ^ (row & 7u)) << 4);
             const uint32_t r4[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
@@ -764,14 +841,14 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
         // is looked through; above 128 rows the first warpgroup does it for both.
         if ((masked || copies > 1u) && !(w.two && t == 1u)) {
           const uint32_t load = base + v_order(w.two, j, n);
-          if (!wait_all(full(load % NS), load / NS, B2G_SITE_FULL)) break;
+          wait_all(full(load % NS), load / NS, B2G_SITE_FULL);
           const bool mine = clear_odd_values<D, kBF16>(
               sbase + TP::kRingOff + (load % NS) * TP::kTile + row * 128u, lane);
           const uint32_t found = __ballot_sync(0xffffffffu, mine);
           if (found != 0u) fence_proxy_async_smem();
           odd |= found;
         }
-        if (!wait_all(s_full(t), step, B2G_SITE_ACC_FULL)) break;
+        wait_all(s_full(t), step, B2G_SITE_ACC_FULL);
         tc_fence_after();
         if (j + stride >= n && lane == 0) odd_words[(ic & 1u) * 8u + t * 4u + quarter] = odd;
         uint32_t seen[4] = {~0u, ~0u, ~0u, ~0u};
@@ -793,11 +870,10 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
           tree_softmax<D, kBF16, 1>(s_col, o_col, c0, p.scale_log2, masked, seen, first, m_run,
                                     l_run, p_full(t, 0), p_full(t, 1), lane);
       }
-      if (!alive) break;
 
       const bool active = t < w.slots;
       if (active) {
-        if (!wait_all(o_done(t), ti, B2G_SITE_ACC_FULL)) break;
+        wait_all(o_done(t), ti, B2G_SITE_ACC_FULL);
         tc_fence_after();
         ++ti;
       }
@@ -857,14 +933,14 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
         // the copies and the two warpgroups meet: maxima and sums first, then O in
         // column chunks through shared memory, already scaled by the writers
         ml[(t * 4u + quarter) * 32u + lane] = make_float2(m_run, l_run);
-        if (!meet()) break;
+        meet();
         const volatile uint32_t* ow = odd_words + (ic & 1u) * 8u;
         bool any_odd = (ow[0] | ow[1] | ow[2] | ow[3]) != 0u;
         if (w.slots == 2u) any_odd |= (ow[4] | ow[5] | ow[6] | ow[7]) != 0u;
         const uint32_t parts = w.slots * copies;  // at most eight
         // warp of part c that holds this row, or row r
         auto warp_of = [&](uint32_t c, uint32_t r) {
-          return (c / copies) * 4u + (c % copies) * per + (r >> 5);
+          return ((c >> lc) << 2) + ((c & (copies - 1u)) << (2u - lc)) + (r >> 5);
         };
         float m_tot = -INFINITY, l_tot = 0.0f;
         {
@@ -885,12 +961,14 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
         // A round takes 32 columns, or as many as the buffer holds of fewer rows: it
         // is [8 warps][row][columns], the float4s of a row permuted so that eight
         // rows at once spread over the banks.
-        const uint32_t wrows = w.rows <= 8 ? 8u : w.rows <= 16 ? 16u : 32u;  // rows of a warp
-        const uint32_t cols = min(static_cast<uint32_t>(D), TP::kTile / (8u * 4u) / wrows);
-        const uint32_t vecs = cols / 4u;  // a power of two
+        const uint32_t lw = w.rows <= 8 ? 3u : w.rows <= 16 ? 4u : 5u;  // log2 rows of a warp
+        constexpr uint32_t kLogTile = D == 128 ? 15 : 14;
+        static_assert(TP::kTile == 1u << kLogTile, "join buffer");
+        const uint32_t lv = min(D == 128 ? 5u : 4u, kLogTile - 3u - 4u - lw);  // log2 float4s of a round
+        const uint32_t vecs = 1u << lv, cols = vecs * 4u;
         const uint32_t buf = sbase + TP::kJoinOff;
         auto at = [&](uint32_t wq, uint32_t r, uint32_t v) {
-          return buf + ((wq * wrows + r) * vecs + (v ^ (r & (vecs - 1u) & 7u))) * 16u;
+          return buf + ((((wq << lw) + r) << lv) + (v ^ (r & (vecs - 1u) & 7u))) * 16u;
         };
         for (uint32_t d = 0; d < static_cast<uint32_t>(D); d += cols) {
           if (active) {
@@ -916,39 +994,48 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
               if (lane == 0) mbar_arrive(o_free(t));
             }
           }
-          if (!meet()) break;
-          // four columns of one row to a thread
-          for (uint32_t i = threadIdx.x - 64u; i < static_cast<uint32_t>(w.rows) * vecs; i += 256u) {
-            const uint32_t r = i / vecs, v = i % vecs;
+          meet();
+          // four columns of a row to a thread: neighbours along the row where it goes to
+          // O, neighbouring rows where it goes to the unfinished ones
+          auto sum_of = [&](uint32_t r, uint32_t v) {
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (uint32_t c = 0; c < 8; ++c) {
-              if (c < parts) {
-                uint32_t x[4];
-                ld_shared_v4(at(warp_of(c, r), r & 31u, v), x);
-                sum.x += __uint_as_float(x[0]);
-                sum.y += __uint_as_float(x[1]);
-                sum.z += __uint_as_float(x[2]);
-                sum.w += __uint_as_float(x[3]);
-              }
+#pragma unroll 2
+            for (uint32_t c = 0; c < parts; ++c) {
+              uint32_t x[4];
+              ld_shared_v4(at(warp_of(c, r), r & 31u, v), x);
+              sum.x += __uint_as_float(x[0]);
+              sum.y += __uint_as_float(x[1]);
+              sum.z += __uint_as_float(x[2]);
+              sum.w += __uint_as_float(x[3]);
             }
-            const int32_t g = w.row0 + static_cast<int32_t>(r), tk = g / p.G;
-            const int32_t col = static_cast<int32_t>(d + 4u * v);
-            if (whole) {
+            return sum;
+          };
+          if (whole) {
+            for (uint32_t i = threadIdx.x - 64u; i < static_cast<uint32_t>(w.rows) << lv; i += 256u) {
+              const uint32_t r = i >> lv, v = i & (vecs - 1u);
+              const float4 sum = sum_of(r, v);
+              const int32_t g = w.row0 + static_cast<int32_t>(r), tk = g / p.G;
+              const int32_t col = static_cast<int32_t>(d + 4u * v);
               T* dst = static_cast<T*>(p.O) + static_cast<int64_t>(w.e.first + tk) * p.o_t +
-                       (w.hk * p.G + g % p.G) * p.o_h + col;
+                       (w.hk * p.G + g - tk * p.G) * p.o_h + col;
               *reinterpret_cast<uint2*>(dst) =
                   make_uint2(pack2<kBF16>(sum.x, sum.y), pack2<kBF16>(sum.z, sum.w));
               if (any_odd) add_odd_cache_values<D, T>(p, w, tk, col, 4, dst);
-            } else {
-              float4* dst = part + (col / 4) * p.part_rows + r;
-              *dst = sum;
-              if (any_odd) add_odd_cache_values<D, T>(p, w, tk, col, 4, &dst->x);
+            }
+          } else {
+            for (uint32_t v = warp - 2u; v < vecs; v += 8u) {
+              for (uint32_t r = lane; r < static_cast<uint32_t>(w.rows); r += 32u) {
+                const int32_t col = static_cast<int32_t>(d + 4u * v);
+                float4* dst = part + (col / 4) * p.part_rows + r;
+                *dst = sum_of(r, v);
+                if (any_odd)
+                  add_odd_cache_values<D, T>(p, w, (w.row0 + static_cast<int32_t>(r)) / p.G, col, 4,
+                                             &dst->x);
+              }
             }
           }
-          if (!meet()) break;  // the buffer is free again
+          meet();  // the buffer is free again
         }
-        if (!alive) break;
       }
       if (!whole) {
         OpenBlock b;
@@ -967,7 +1054,8 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
     // The blocks that this share had a part of: this CTA's parts are published, and
     // when all of a block's are, each of its CTAs joins a slice of the block's
     // values, in the order of the shares.
-    if (alive && (open_first.owner >= 0 || open_last.owner >= 0) && meet()) {
+    if (open_first.owner >= 0 || open_last.owner >= 0) {
+      meet();
       const int32_t owner = lane == 0 ? open_first.owner : open_last.owner;
       if (warp == 2u && lane < 2u && owner >= 0) {
         __threadfence();
@@ -975,13 +1063,13 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
       }
     }
 #pragma unroll 1
-    for (int slot = 0; alive && slot < 2; ++slot) {
+    for (int slot = 0; slot < 2; ++slot) {
       const OpenBlock b = slot == 0 ? open_first : open_last;
       if (b.owner < 0) continue;
-      uint32_t* count = p.counters + 2 * b.owner;
-      bool there = true;
-      if (lane == 0) {
+      if (warp == 2u && lane == 0) {
+        uint32_t* count = p.counters + 2 * b.owner;
         const uint64_t t0 = globaltimer_ns();
+        bool there = true;
         while (ld_acquire_gpu(count) < static_cast<uint32_t>(b.parts)) {
           if (*abort_flag != 0u || globaltimer_ns() - t0 > p.timeout_ns) {
             fmha_report(p, B2G_STATUS_TIMEOUT | B2G_SITE_FLAG);
@@ -990,70 +1078,22 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
             break;
           }
         }
-      }
-      if (!__all_sync(0xffffffffu, there)) {
-        alive = false;
-        break;
-      }
-      // a float4 of one row to a thread, neighbours in the row index
-      const int32_t k = me - b.owner;
-      const int64_t all = static_cast<int64_t>(b.rows) * (D / 4);
-      const int64_t stop = all * (k + 1) / b.parts;
-      for (int64_t i = all * k / b.parts + (threadIdx.x - 64u); i < stop; i += 256) {
-        const int32_t r = static_cast<int32_t>(i % b.rows), v = static_cast<int32_t>(i / b.rows);
-        float m = -INFINITY, l = 0.0f;
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int32_t c0 = 0; c0 < b.parts; c0 += kJoinBatch) {
-          float2 x[kJoinBatch];
-          float4 o[kJoinBatch];
-#pragma unroll
-          for (int32_t c = 0; c < kJoinBatch; ++c) {
-            x[c] = make_float2(-INFINITY, 0.0f);
-            o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (c0 + c < b.parts) {
-              const int64_t id = c0 + c == 0 ? 2 * b.owner + 1 : 2 * (b.owner + c0 + c);
-              x[c] = __ldcg(&p.part_ml[id * p.part_rows + r]);
-              o[c] = __ldcg(reinterpret_cast<const float4*>(p.part) +
-                            (id * (D / 4) + v) * p.part_rows + r);
-            }
-          }
-          float top = m;
-#pragma unroll
-          for (int32_t c = 0; c < kJoinBatch; ++c) top = fmaxf(top, x[c].x);
-          if (top == -INFINITY) continue;  // nothing seen so far
-          const float was = fast_exp2(m - top);
-          l *= was;
-          sum = make_float4(sum.x * was, sum.y * was, sum.z * was, sum.w * was);
-          m = top;
-#pragma unroll
-          for (int32_t c = 0; c < kJoinBatch; ++c) {
-            if (c0 + c >= b.parts) continue;
-            const float f = fast_exp2(x[c].x - m);
-            l = fmaf(x[c].y, f, l);
-            sum.x = fmaf(o[c].x, f, sum.x);
-            sum.y = fmaf(o[c].y, f, sum.y);
-            sum.z = fmaf(o[c].z, f, sum.z);
-            sum.w = fmaf(o[c].w, f, sum.w);
-          }
-        }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const int32_t g = b.row0 + r, tk = b.first + g / p.G, h = b.hk * p.G + g % p.G;
-        T* dst = static_cast<T*>(p.O) + static_cast<int64_t>(tk) * p.o_t + h * p.o_h + 4 * v;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<kBF16>(sum.x * inv, sum.y * inv),
-                                                    pack2<kBF16>(sum.z * inv, sum.w * inv));
-        if (v == 0 && p.lse != nullptr)
-          p.lse[static_cast<int64_t>(h) * p.tokens + tk] =
-              l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.693147180559945309f;
-      }
-      // the last CTA to have read the parts leaves both counts at zero
-      if (!meet()) break;
-      if (warp == 2u && lane == 0) {
-        __threadfence();
-        if (atomicAdd(&count[1], 1u) + 1u == static_cast<uint32_t>(b.parts)) {
+        // the last CTA to have seen the count leaves both words at zero
+        if (there && atomicAdd(&count[1], 1u) + 1u == static_cast<uint32_t>(b.parts)) {
           count[0] = 0u;
           count[1] = 0u;
         }
+        __threadfence();
       }
+      meet();
+      if (*abort_flag != 0u) continue;
+      const int32_t k = me - b.owner, w8 = static_cast<int32_t>(warp) - 2, ln = static_cast<int32_t>(lane);
+      if (b.parts <= 2)
+        join_parts<D, kBF16, 4, 2>(p, b, k, w8, ln);
+      else if (b.parts <= 4)
+        join_parts<D, kBF16, 2, 4>(p, b, k, w8, ln);
+      else
+        join_parts<D, kBF16, 1, 12>(p, b, k, w8, ln);
     }
   }
 
