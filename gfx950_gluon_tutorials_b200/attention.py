@@ -35,6 +35,7 @@ _DT = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
 HEAD_DIMS = (64, 128)
 BLOCK_M, BLOCK_N = 128, 128   # query rows per CTA, keys per tile
 KERNEL_NAME = "fmha_fwd_kernel"
+_I64x8, _I64x10 = ctypes.c_int64 * 8, ctypes.c_int64 * 10
 
 
 class MetaData:
@@ -177,11 +178,22 @@ def _packed(t: torch.Tensor) -> bool:
     """Whether a (tokens, heads, dim) tensor can be read or written where it lies: unit
     dim stride, 16-byte aligned base and rows."""
     s0, s1, s2 = t.stride()
-    return s2 == 1 and s0 > 0 and s1 > 0 and not ((s0 | s1) & 7) and not t.data_ptr() & 15
+    return s2 == 1 and s0 > 0 < s1 and not ((s0 | s1) & 7 or t.data_ptr() & 15)
 
 
 def _readable(t: torch.Tensor) -> torch.Tensor:
     return t if _packed(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def _with_workspace(call, args: tuple, dev: torch.device, nbytes) -> int:
+    """``call(*args, workspace, its size, status, stream)`` with the stream's workspace as it
+    is; asks how large it has to be only when the call finds it too small."""
+    ws, status, stream = workspace(0, dev), status_tensor(dev).data_ptr(), _stream_handle(dev)
+    rc = call(*args, ws.data_ptr(), ws.numel(), status, stream)
+    if rc == _lib.EWORKSPACE:
+        ws = workspace(nbytes(), dev)
+        rc = call(*args, ws.data_ptr(), ws.numel(), status, stream)
+    return rc
 
 
 def _check_packed(q: torch.Tensor, hk: int, o, lse) -> tuple[int, int, int, torch.Tensor]:
@@ -234,15 +246,13 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
     out = o if _packed(o) else torch.empty(o.shape, dtype=o.dtype, device=dev)
     if out is not o:
         out.copy_(o)  # rows past the last prompt keep what o holds
-    strides = (ctypes.c_int64 * 8)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2],
-                                   *out.stride()[:2])
+    strides = _I64x8(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *out.stride()[:2])
     handle = _lib.lib()
-    ws = workspace(handle.b2g_attention_prefill_workspace_bytes(prompts, tokens, hq), dev)
-    rc = handle.b2g_attention_prefill(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), strides, cu_seqlens.data_ptr(),
-        prompts, tokens, hq, k.shape[1], dim, _DT[q.dtype],
-        dim ** -0.5 if sm_scale is None else sm_scale, None if lse is None else lse.data_ptr(),
-        ws.data_ptr(), ws.numel(), status_tensor(dev).data_ptr(), _stream_handle(dev))
+    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), strides,
+            cu_seqlens.data_ptr(), prompts, tokens, hq, k.shape[1], dim, _DT[q.dtype],
+            dim ** -0.5 if sm_scale is None else sm_scale, None if lse is None else lse.data_ptr())
+    rc = _with_workspace(handle.b2g_attention_prefill, args, dev,
+                         lambda: handle.b2g_attention_prefill_workspace_bytes(prompts, tokens, hq))
     _lib.check(rc, "b2g_attention_prefill")
     if out is not o:
         o.copy_(out)
@@ -282,8 +292,10 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if block_tables.dim() != 2 or block_tables.dtype != torch.int32:
         raise ValueError("block_tables must be a 2-D int32 tensor")
     requests, max_pages = block_tables.shape
-    if max_pages > 1 and block_tables.stride(1) != 1:
+    table_stride, column_stride = block_tables.stride()
+    if max_pages > 1 and column_stride != 1:
         block_tables = block_tables.contiguous()
+        table_stride = max_pages
     seq_lens = _int_vector(seq_lens, requests, torch.int32, "seq_lens")
     cu_seqlens = _int_vector(cu_seqlens, requests + 1, torch.int32, "cu_seqlens")
     words = 0
@@ -300,17 +312,17 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     out = o if _packed(o) else torch.empty(o.shape, dtype=o.dtype, device=dev)
     if out is not o:
         out.copy_(o)  # rows past the last request keep what o holds
-    strides = (ctypes.c_int64 * 10)(*q.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3],
-                                    *out.stride()[:2])
+    strides = _I64x10(*q.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3],
+                      *out.stride()[:2])
     handle = _lib.lib()
-    ws = workspace(handle.b2g_attention_tree_workspace_bytes(requests, tokens, hq, hk, dim), dev)
-    rc = handle.b2g_attention_tree(
-        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), strides,
-        block_tables.data_ptr(), block_tables.stride(0), max_pages, seq_lens.data_ptr(),
-        cu_seqlens.data_ptr(), None if tree_mask is None else tree_mask.data_ptr(), words,
-        requests, tokens, hq, hk, dim, pages, page, _DT[q.dtype],
-        dim ** -0.5 if sm_scale is None else sm_scale, None if lse is None else lse.data_ptr(),
-        ws.data_ptr(), ws.numel(), status_tensor(dev).data_ptr(), _stream_handle(dev))
+    args = (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), strides,
+            block_tables.data_ptr(), table_stride, max_pages, seq_lens.data_ptr(),
+            cu_seqlens.data_ptr(), None if tree_mask is None else tree_mask.data_ptr(), words,
+            requests, tokens, hq, hk, dim, pages, page, _DT[q.dtype],
+            dim ** -0.5 if sm_scale is None else sm_scale, None if lse is None else lse.data_ptr())
+    rc = _with_workspace(handle.b2g_attention_tree, args, dev,
+                         lambda: handle.b2g_attention_tree_workspace_bytes(requests, tokens, hq,
+                                                                           hk, dim))
     _lib.check(rc, "b2g_attention_tree")
     if out is not o:
         o.copy_(out)

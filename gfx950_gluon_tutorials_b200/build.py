@@ -20,7 +20,7 @@ INCLUDE = os.path.join(REPO_DIR, "include")
 LIB_PATH = os.path.join(PKG_DIR, "libb2g.so")
 
 SOURCES = ["capi.cu", "pack.cu", "noalloc.cu", "attention.cu",
-           "attention_tree.cu", "kvcache.cu"]
+           "attention_prefill.cu", "attention_tree.cu", "kvcache.cu"]
 HEADERS = ["ptx.cuh", "sched.h", "gemm_kernel.cuh", "skinny_kernel.cuh", "pack.cuh",
            "capi_internal.h", "attention_common.cuh"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -25,19 +25,6 @@
 // from the caller's strides, so bhsd and bshd layouts and GQA (query head h
 // reads key/value head h / (HQ / HK)) need no copies; keys and query rows
 // past the sequence ends are zero-filled by TMA and masked.
-//
-// kPacked = true is causal attention over packed prompts (attention_prefill) with
-// the same CTA. Row i of a prompt sees keys j <= i, so a 128-row tile that starts
-// at row m of its prompt needs m / 128 + 1 KV tiles, of which only the last is
-// masked, by a triangle (which hides the keys past the prompt's end too: they lie
-// after every row that is stored). Items are the 256-row blocks of all prompts,
-// listed by a planning kernel (packed_plan_kernel) in order of falling work and
-// dealt to the CTAs in turns of alternating direction, which evens out their sums.
-//
-// What is masked must not count whatever it holds, and 0 * NaN would: the keys of
-// the last KV tile may be another prompt's, or later tokens of the same one. So
-// the softmax warps look through that tile of V before its PV product, set what
-// is not finite to zero, and the epilogue adds it to the rows that do see it.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -46,7 +33,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <climits>
 #include <cmath>
 #include <cstdint>
 #include <cstring>
@@ -75,11 +61,6 @@ struct alignas(64) FmhaParams {
   int32_t B, HQ, HK, S_q, S_k;
   float scale_log2;           // sm_scale * log2(e)
   uint64_t timeout_ns;
-  // packed form: S_q = S_k = tokens in all, B = 1
-  const int4* plan;           // {first token of the block, its row in the prompt, prompt's rows, 0}
-  const int32_t* plan_count;  // entries in plan; each stands for HQ items
-  const void* V;              // with its strides, for the rows that see values that are not finite
-  int64_t v_sh, v_ss;
 };
 
 // Shared memory and TMEM plan of one CTA: two 128-row query tiles (Q0, Q1),
@@ -101,8 +82,7 @@ struct FmhaPlan {
   // (tile, key half), o_done[2], q_empty, o_free[2]
   static constexpr uint32_t kNumBars = 1 + 4 * kStages + 11;
   static constexpr uint32_t kMiscOff = kBarOff + kNumBars * 8;  // tmem slot, abort flag
-  static constexpr uint32_t kOddOff = kMiscOff + 16;  // packed form: odd-value masks [2 tiles][2 items][4 warps]
-  static constexpr uint32_t kBytes = kOddOff + 64;
+  static constexpr uint32_t kBytes = kMiscOff + 16;
   static constexpr uint32_t kDynBytes = kBytes + 1024;  // + alignment slack
   // TMEM columns: S_t = 128 t (128 fp32), P_t = S_t + 64 (128 x 16-bit),
   // O_t = 256 + 128 t (D fp32)
@@ -112,22 +92,7 @@ struct FmhaPlan {
   static_assert(kDynBytes <= 232448, "shared memory");
 };
 
-// Adds the values that are not finite of tokens [t0, t1) of V, which the product
-// left out, to a stored row of O. The weights that multiply them are positive, so
-// they carry over as they are.
-template <int D, typename T>
-__device__ __noinline__ void add_odd_values(const FmhaParams& p, int32_t t0, int32_t hk, int32_t t1,
-                                            T* orow) {
-  for (int32_t t = t0; t < t1; ++t) {
-    const T* v = static_cast<const T*>(p.V) + hk * p.v_sh + t * p.v_ss;
-    for (int d = 0; d < D; ++d) {
-      const float x = static_cast<float>(v[d]);
-      if (!isfinite(x)) orow[d] = static_cast<T>(static_cast<float>(orow[d]) + x);
-    }
-  }
-}
-
-template <int D, bool kBF16, bool kPacked>
+template <int D, bool kBF16>
 __global__ void __launch_bounds__(FmhaPlan<D>::kThreads, 1)
     fmha_fwd_kernel(const __grid_constant__ FmhaParams p) {
   using FP = FmhaPlan<D>;
@@ -137,50 +102,23 @@ __global__ void __launch_bounds__(FmhaPlan<D>::kThreads, 1)
                                              ~static_cast<uintptr_t>(1023));
   const uint32_t sbase = smem_u32(smem);
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int32_t n_kv = (p.S_k + 127) / 128;
   // Persistent: work items are (256-row query block, query head, batch), the
   // query block fastest, so the CTAs working at one time share K and V in L2.
   const int32_t n_mblk = (p.S_q + 255) / 256;
+  const int32_t n_items = n_mblk * p.HQ * p.B;
   struct Item {
-    int32_t m0, h, b, hk;  // m0: the block's first row, of the sequence or of all tokens
+    int32_t m0, h, b, hk;
     uint32_t tiles;  // query tiles holding rows (1 or 2)
-    int32_t k0;      // the keys' first row: 0, or the prompt's first token
-    int32_t n_kv;    // KV tiles of the last query tile, of both in the dense form
-    int32_t rows;    // rows of the sequence from m0 on
-  };
-  // the item after `item`, this CTA's item number `turn`; the packed form deals
-  // them in alternating direction, so that the list's falling work adds up alike
-  // over the CTAs
-  auto next_item = [&](int32_t item, uint32_t turn) {
-    const int32_t g = static_cast<int32_t>(gridDim.x), c = static_cast<int32_t>(blockIdx.x);
-    if constexpr (kPacked) return item + ((turn & 1u) ? 2 * c + 1 : 2 * (g - c) - 1);
-    return item + g;
   };
   auto item_at = [&](int32_t it) {
     Item w;
-    if constexpr (kPacked) {
-      const int4 e = p.plan[it / p.HQ];
-      w.h = it % p.HQ;
-      w.b = 0;
-      w.m0 = e.x;
-      w.k0 = e.x - e.y;
-      w.rows = e.z - e.y;
-      w.tiles = w.rows > 128 ? 2u : 1u;
-      w.n_kv = e.y / 128 + static_cast<int32_t>(w.tiles);
-    } else {
-      w.m0 = (it % n_mblk) * 256;
-      w.h = (it / n_mblk) % p.HQ;
-      w.b = it / (n_mblk * p.HQ);
-      w.rows = p.S_q - w.m0;
-      w.tiles = w.rows > 128 ? 2u : 1u;
-      w.k0 = 0;
-      w.n_kv = (p.S_k + 127) / 128;
-    }
+    w.m0 = (it % n_mblk) * 256;
+    w.h = (it / n_mblk) % p.HQ;
+    w.b = it / (n_mblk * p.HQ);
     w.hk = w.h / (p.HQ / p.HK);
+    w.tiles = p.S_q - w.m0 > 128 ? 2u : 1u;
     return w;
-  };
-  // KV tiles of query tile t: in the packed form the first of two needs one fewer
-  auto tile_kv = [&](const Item& w, uint32_t t) {
-    return kPacked ? w.n_kv + 1 - static_cast<int32_t>(w.tiles - t) : w.n_kv;
   };
 
   const uint32_t bar0 = sbase + FP::kBarOff;
@@ -229,11 +167,6 @@ __global__ void __launch_bounds__(FmhaPlan<D>::kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-  int32_t n_items = n_mblk * p.HQ * p.B;
-  if constexpr (kPacked) {
-    grid_dependency_wait();  // the plan is complete
-    n_items = *p.plan_count * p.HQ;
-  }
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer --
@@ -244,7 +177,7 @@ __global__ void __launch_bounds__(FmhaPlan<D>::kThreads, 1)
       uint32_t nk = 0, nv = 0;  // K and V loads issued
       bool alive = true;
       for (int32_t item = static_cast<int32_t>(blockIdx.x); alive && item < n_items;
-           item = next_item(item, ic), ++ic) {
+           item += static_cast<int32_t>(gridDim.x), ++ic) {
         const Item w = item_at(item);
         if (ic > 0 && !fmha_wait(q_empty, (ic - 1u) & 1u, abort_flag, p, B2G_SITE_EMPTY)) break;
         mbar_arrive_expect_tx(q_full, w.tiles * FP::kTile);
@@ -252,7 +185,7 @@ __global__ void __launch_bounds__(FmhaPlan<D>::kThreads, 1)
           for (uint32_t r = 0; r < FP::kRegions; ++r)
             tma_load_4d(sbase + FP::kQOff + t * FP::kTile + r * FP::kRegion, &p.tmQ, q_full,
                         r * 64, w.m0 + static_cast<int32_t>(t) * 128, w.h, w.b);
-        for (int32_t j = 0; j < w.n_kv; ++j, ++jg) {
+        for (int32_t j = 0; j < n_kv; ++j, ++jg) {
           const uint32_t s = jg % KS, ph = (jg / KS) & 1u;
           if (!fmha_wait(k_empty(s), ph ^ 1u, abort_flag, p, B2G_SITE_EMPTY)) {
             alive = false;
@@ -261,7 +194,7 @@ __global__ void __launch_bounds__(FmhaPlan<D>::kThreads, 1)
           mbar_arrive_expect_tx(k_full(s), FP::kTile);
           for (uint32_t r = 0; r < FP::kRegions; ++r)
             tma_load_4d(sbase + FP::kKOff + s * FP::kTile + r * FP::kRegion, &p.tmK, k_full(s),
-                        r * 64, w.k0 + j * 128, w.hk, w.b);
+                        r * 64, j * 128, w.hk, w.b);
           ++nk;
           if (!fmha_wait(v_empty(s), ph ^ 1u, abort_flag, p, B2G_SITE_EMPTY)) {
             alive = false;
@@ -270,7 +203,7 @@ __global__ void __launch_bounds__(FmhaPlan<D>::kThreads, 1)
           mbar_arrive_expect_tx(v_full(s), FP::kTile);
           for (uint32_t r = 0; r < FP::kRegions; ++r)
             tma_load_4d(sbase + FP::kVOff + s * FP::kTile + r * FP::kRegion, &p.tmV, v_full(s),
-                        r * 64, w.k0 + j * 128, w.hk, w.b);
+                        r * 64, j * 128, w.hk, w.b);
           ++nv;
         }
       }
@@ -316,10 +249,9 @@ __global__ void __launch_bounds__(FmhaPlan<D>::kThreads, 1)
       uint32_t titems[2] = {0u, 0u};       // items of each tile (phases of o_done, o_free)
       bool alive = true;
       for (int32_t item = static_cast<int32_t>(blockIdx.x); alive && item < n_items;
-           item = next_item(item, ic), ++ic) {
+           item += static_cast<int32_t>(gridDim.x), ++ic) {
         const Item w = item_at(item);
         const uint32_t nt = w.tiles;
-        const int32_t n_kv = w.n_kv;
         if (!fmha_wait(q_full, ic & 1u, abort_flag, p, B2G_SITE_FULL) ||
             !fmha_wait(k_full(jg % KS), (jg / KS) & 1u, abort_flag, p, B2G_SITE_FULL))
           break;
@@ -334,8 +266,7 @@ __global__ void __launch_bounds__(FmhaPlan<D>::kThreads, 1)
         tc_commit<1>(k_empty(jg % KS));
         for (int32_t j = 0; j < n_kv; ++j, ++jg) {
           const uint32_t s = jg % KS, ph = (jg / KS) & 1u;
-          const bool any_next = j + 1 < n_kv;
-          bool k_ready = false;  // K of the next step is in shared memory
+          const bool has_next = j + 1 < n_kv;
           const uint32_t s1 = (jg + 1) % KS, ph1 = ((jg + 1) / KS) & 1u;
           if (!fmha_wait(v_full(s), ph, abort_flag, p, B2G_SITE_FULL)) {
             alive = false;
@@ -343,8 +274,6 @@ __global__ void __launch_bounds__(FmhaPlan<D>::kThreads, 1)
           }
           const uint32_t v_base = sbase + FP::kVOff + s * FP::kTile;
           for (uint32_t t = 0; alive && t < nt; ++t) {
-            if (kPacked && j >= tile_kv(w, t)) continue;  // the first tile's last step is behind
-            const bool has_next = kPacked ? j + 1 < tile_kv(w, t) : any_next;
             const uint32_t p_col = tmem_base + FP::kS + t * FP::kTileCols + FP::kP;
             // the previous item's epilogue must have read this tile's O
             if (j == 0 && titems[t] > 0 &&
@@ -378,11 +307,10 @@ __global__ void __launch_bounds__(FmhaPlan<D>::kThreads, 1)
               ++titems[t];
               continue;
             }
-            if (!k_ready && !fmha_wait(k_full(s1), ph1, abort_flag, p, B2G_SITE_FULL)) {
+            if (t == 0 && !fmha_wait(k_full(s1), ph1, abort_flag, p, B2G_SITE_FULL)) {
               alive = false;
               break;
             }
-            k_ready = true;
             tc_fence_after();
             issue_s(t, s1);
             tc_commit<1>(s_full(t));
@@ -392,7 +320,7 @@ __global__ void __launch_bounds__(FmhaPlan<D>::kThreads, 1)
           if (!alive) break;
           if (j + 2 == n_kv) tc_commit<1>(q_empty);  // the item's last S MMAs are issued
           tc_commit<1>(v_empty(s));
-          if (any_next) tc_commit<1>(k_empty(s1));
+          if (has_next) tc_commit<1>(k_empty(s1));
         }
       }
       // all MMAs issued by this thread finish before TMEM can be freed
@@ -416,52 +344,20 @@ __global__ void __launch_bounds__(FmhaPlan<D>::kThreads, 1)
       const uint32_t o_col = taddr + FP::kO + t * FP::kTileCols;
       const float sl2 = p.scale_log2;
       uint32_t step = 0, ti = 0;  // this tile's steps and items (barrier phases)
-      uint32_t jg_next = 0, ic = 0;  // K/V steps and items of the CTA
-      // packed form, [item & 1][warp]: which of a warp's 32 rows of the tile's last V tile
-      // hold values that are not finite
-      auto odd_masks = [&](uint32_t tile, uint32_t parity) {
-        return reinterpret_cast<volatile uint32_t*>(smem + FP::kOddOff) + (tile * 2u + (parity & 1u)) * 4u;
-      };
       bool alive = true;
       for (int32_t item = static_cast<int32_t>(blockIdx.x); alive && item < n_items;
-           item = next_item(item, ic), ++ic) {
+           item += static_cast<int32_t>(gridDim.x)) {
       const Item w = item_at(item);
-      const uint32_t jg = jg_next;
-      jg_next += static_cast<uint32_t>(w.n_kv);
       if (t >= w.tiles) continue;
-      const int32_t n_kv = tile_kv(w, t);
-      bool odd_before = false;  // the first tile's last V tile, which this one sees whole
       float m_run = -INFINITY;  // exponent offset, log2 units (a running max of s * sl2)
       float l_run = 0.0f;       // running sum of exp2(s * sl2 - m_run)
       for (int32_t j = 0; j < n_kv; ++j, ++step) {
-        const bool diagonal = kPacked && j + 1 == n_kv;
-        uint32_t odd = 0;
-        if (diagonal) {
-          const uint32_t vs = (jg + static_cast<uint32_t>(j)) % KS;
-          if (!__all_sync(0xffffffffu,
-                          fmha_wait(v_full(vs), ((jg + static_cast<uint32_t>(j)) / KS) & 1u,
-                                    abort_flag, p, B2G_SITE_FULL))) {
-            alive = false;
-            break;
-          }
-          const bool mine =
-              clear_odd_values<D, kBF16>(sbase + FP::kVOff + vs * FP::kTile + row * 128u, lane);
-          odd = __ballot_sync(0xffffffffu, mine);
-          if (odd != 0u) fence_proxy_async_smem();  // the PV product reads the zeros
-        }
         if (!__all_sync(0xffffffffu, fmha_wait(s_full(t), step & 1u,
                                                abort_flag, p, B2G_SITE_ACC_FULL))) {
           alive = false;
           break;
         }
         tc_fence_after();
-        if (diagonal) {
-          if (lane == 0) odd_masks(t, ti)[quarter] = odd;
-          if (t == 1) {  // the first tile takes part in every item, so its parity is ic's
-            const volatile uint32_t* m = odd_masks(0, ic);
-            odd_before = (m[0] | m[1] | m[2] | m[3]) != 0u;
-          }
-        }
         uint32_t s[128];
         {
           uint32_t (&s0)[32] = *reinterpret_cast<uint32_t(*)[32]>(&s[0]);
@@ -474,9 +370,8 @@ __global__ void __launch_bounds__(FmhaPlan<D>::kThreads, 1)
           tmem_ld_32x32b_x32(s_col + 96u, s3);
           tmem_wait_ld();
         }
-        // keys past S_k (zero-filled by TMA) or after this row take no part
-        const int32_t valid = kPacked ? (diagonal ? static_cast<int32_t>(row) + 1 : 128)
-                                      : p.S_k - j * 128;
+        // keys past S_k (zero-filled by TMA) take no part
+        const int32_t valid = p.S_k - j * 128;
         if (valid < 128) {
 #pragma unroll
           for (int c = 0; c < 128; ++c)
@@ -519,9 +414,7 @@ __global__ void __launch_bounds__(FmhaPlan<D>::kThreads, 1)
         }
 
         const float2 sl2x2 = make_float2(sl2, sl2);
-        // a row whose scores are all -inf so far keeps weights of zero
-        const float off = kPacked && m_new == -INFINITY ? 0.0f : -m_new;
-        const float2 negm = make_float2(off, off);
+        const float2 negm = make_float2(-m_new, -m_new);
         // Exponentials, 32 columns at a time: chunks 0 and 1 straight from the
         // registers of the max pass, chunks 2 and 3 reloaded from TMEM (each load
         // in flight while the previous chunk is exponentiated), so that few
@@ -601,8 +494,8 @@ __global__ void __launch_bounds__(FmhaPlan<D>::kThreads, 1)
       if (lane == 0) mbar_arrive(o_free(t));
       ++ti;
       const int32_t q_row = w.m0 + static_cast<int32_t>(t * 128u + row);
-      if (kPacked ? static_cast<int32_t>(t * 128u + row) < w.rows : q_row < p.S_q) {
-        const float inv_l = kPacked && l_run == 0.0f ? 0.0f : 1.0f / l_run;
+      if (q_row < p.S_q) {
+        const float inv_l = 1.0f / l_run;
         using OutT = typename std::conditional<kBF16, __nv_bfloat16, __half>::type;
         OutT* orow = static_cast<OutT*>(p.O) + static_cast<int64_t>(w.b) * p.o_sb +
                      static_cast<int64_t>(w.h) * p.o_sh + static_cast<int64_t>(q_row) * p.o_ss;
@@ -615,11 +508,6 @@ __global__ void __launch_bounds__(FmhaPlan<D>::kThreads, 1)
           u.z = pack2<kBF16>(__uint_as_float(o[8 * v + 4]) * inv_l, __uint_as_float(o[8 * v + 5]) * inv_l);
           u.w = pack2<kBF16>(__uint_as_float(o[8 * v + 6]) * inv_l, __uint_as_float(o[8 * v + 7]) * inv_l);
           dst[v] = u;
-        }
-        if constexpr (kPacked) {
-          const volatile uint32_t* m = odd_masks(t, ti - 1u);
-          if (odd_before || (m[0] | m[1] | m[2] | m[3]) != 0u)
-            add_odd_values<D>(p, w.m0, w.hk, q_row + 1, orow);
         }
         if (p.lse != nullptr) {
           // natural-log log-sum-exp of the scaled scores of this row
@@ -643,10 +531,10 @@ __global__ void __launch_bounds__(FmhaPlan<D>::kThreads, 1)
 // ------------------------------------------------------------------ host --
 namespace {
 
-template <int D, bool kBF16, bool kPacked>
-int launch_fmha(const FmhaParams& prm, int64_t items, cudaStream_t stream) {
+template <int D, bool kBF16>
+int launch_fmha(const FmhaParams& prm, int batch, int heads_q, int seqlen_q, cudaStream_t stream) {
   using FP = FmhaPlan<D>;
-  auto kern = fmha_fwd_kernel<D, kBF16, kPacked>;
+  auto kern = fmha_fwd_kernel<D, kBF16>;
   // At least half the SM's shared memory, so that two CTAs never share an SM
   // (each holds all 512 TMEM columns).
   const uint32_t dyn = FP::kDynBytes > 120u * 1024u ? FP::kDynBytes : 120u * 1024u;
@@ -663,125 +551,14 @@ int launch_fmha(const FmhaParams& prm, int64_t items, cudaStream_t stream) {
     attr_set[dev].store(true);
   }
   // persistent: one CTA per SM, looping over the (query block, head, batch) items
+  const int64_t items = static_cast<int64_t>((seqlen_q + 255) / 256) * heads_q * batch;
   const int sms = current_device_sms();
   if (sms <= 0) return B2G_ENODEVICE;
   if (items > INT32_MAX) return B2G_ESHAPE;
   const dim3 grid(static_cast<unsigned>(items < sms ? items : sms), 1, 1);
-  cudaError_t e;
-  if constexpr (kPacked) {
-    // set up while the planning kernel runs; grid_dependency_wait orders the rest
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(FP::kThreads, 1, 1);
-    cfg.dynamicSmemBytes = dyn;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kern, prm);
-    if (e != cudaSuccess) cudaGetLastError();
-  } else {
-    kern<<<grid, FP::kThreads, dyn, stream>>>(prm);
-    e = cudaGetLastError();
-  }
+  kern<<<grid, FP::kThreads, dyn, stream>>>(prm);
+  const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? B2G_OK : static_cast<int>(e);
-}
-
-}  // namespace
-
-// ------------------------------------------------------------ packed plan --
-// The 256-row blocks of all prompts in order of falling work (KV tiles of their
-// last query tile), by a counting sort over kPlanLevels work levels: blocks of
-// equal level come in any order, and longer prompts than the levels reach share
-// the first. One CTA; latency-bound (three passes over the offsets). The order
-// only decides which CTA works when, never a result.
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanLevels = 4096;  // KV tiles of 128 keys: half a million tokens
-
-struct PackedPlanParams {
-  const int32_t* cu;
-  int4* plan;
-  int32_t* count;
-  int* status;
-  int32_t prompts, tokens;
-  int32_t capacity;  // of plan; only offsets that decrease can ask for more
-};
-
-__global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PackedPlanParams p) {
-  __shared__ int32_t level[kPlanLevels];  // blocks of a level, then where they go
-  __shared__ int32_t warp_sum[kPlanThreads / 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  grid_launch_dependents();
-  for (int i = threadIdx.x; i < kPlanLevels; i += kPlanThreads) level[i] = 0;
-  __syncthreads();
-  // offsets are 0 <= cu[0] <= cu[1] <= ... <= tokens; others are cut to that
-  auto prompt = [&](int b, int32_t& begin, int32_t& rows) {
-    const int32_t lo = p.cu[b], hi = p.cu[b + 1];
-    begin = min(max(lo, 0), p.tokens);
-    rows = min(max(hi, begin), p.tokens) - begin;
-    if ((lo < 0 || hi < lo || hi > p.tokens) && p.status != nullptr)
-      atomicCAS(p.status, 0, B2G_STATUS_TOKENS);
-  };
-  // a warp to a prompt, a lane to a block; falling work is rising level here
-  auto level_of = [](int32_t row, int32_t rows) {
-    const int32_t kv = row / 128 + (rows - row > 128 ? 2 : 1);
-    return kPlanLevels - min(kv, kPlanLevels);
-  };
-  for (int b = warp; b < p.prompts; b += kPlanThreads / 32) {
-    int32_t begin, rows;
-    prompt(b, begin, rows);
-    for (int32_t row = lane * 256; row < rows; row += 32 * 256)
-      atomicAdd(&level[level_of(row, rows)], 1);
-  }
-  __syncthreads();
-  // exclusive sums over the levels, four to a thread
-  constexpr int kPer = kPlanLevels / kPlanThreads;
-  int32_t mine[kPer], sum = 0;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    mine[i] = sum;
-    sum += level[threadIdx.x * kPer + i];
-  }
-  int32_t upto = sum;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int32_t u = __shfl_up_sync(0xffffffffu, upto, d);
-    if (lane >= d) upto += u;
-  }
-  if (lane == 31) warp_sum[warp] = upto;
-  __syncthreads();
-  int32_t base = upto - sum, total = 0;
-  for (int w = 0; w < kPlanThreads / 32; ++w) {
-    if (w < warp) base += warp_sum[w];
-    total += warp_sum[w];
-  }
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) level[threadIdx.x * kPer + i] = base + mine[i];
-  if (threadIdx.x == 0) *p.count = min(total, p.capacity);
-  __syncthreads();
-  for (int b = warp; b < p.prompts; b += kPlanThreads / 32) {
-    int32_t begin, rows;
-    prompt(b, begin, rows);
-    for (int32_t row = lane * 256; row < rows; row += 32 * 256) {
-      const int32_t at = atomicAdd(&level[level_of(row, rows)], 1);
-      if (at < p.capacity) p.plan[at] = make_int4(begin + row, row, rows, 0);
-    }
-  }
-}
-
-namespace {
-
-// Most blocks that `tokens` in `prompts` can have: one for every 256 tokens and a
-// ragged one for each prompt.
-int64_t packed_blocks(int prompts, int64_t tokens) {
-  return tokens / 256 + std::min<int64_t>(prompts, tokens);
-}
-
-size_t packed_workspace(int prompts, int64_t tokens, int sms) {
-  return workspace_flag_bytes(sms) + 256 +
-         static_cast<size_t>(packed_blocks(prompts, tokens)) * sizeof(int4);
 }
 
 }  // namespace
@@ -837,88 +614,11 @@ extern "C" int b2g_attention_fwd(const void* q, const void* k, const void* v, vo
   prm.timeout_ns = wait_timeout_ns();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = dtype == B2G_DT_BF16;
-  const int64_t items = static_cast<int64_t>((seqlen_q + 255) / 256) * heads_q * batch;
   if (head_dim == 128)
-    return bf16 ? launch_fmha<128, true, false>(prm, items, s)
-                : launch_fmha<128, false, false>(prm, items, s);
-  return bf16 ? launch_fmha<64, true, false>(prm, items, s)
-              : launch_fmha<64, false, false>(prm, items, s);
-}
-
-extern "C" size_t b2g_attention_prefill_workspace_bytes(int prompts, int64_t tokens, int heads_q) {
-  (void)heads_q;
-  const int sms = b2g::current_device_sms();
-  if (sms <= 0 || prompts < 0 || tokens < 0) return 0;
-  return b2g::packed_workspace(prompts, tokens, sms);
-}
-
-extern "C" int b2g_attention_prefill(const void* q, const void* k, const void* v, void* o,
-                                     const int64_t* strides, const int32_t* cu_seqlens,
-                                     int prompts, int64_t tokens, int heads_q, int heads_k,
-                                     int head_dim, int dtype, float sm_scale, float* lse,
-                                     void* workspace, size_t workspace_bytes, int* status,
-                                     void* stream) {
-  using namespace b2g;
-  if (tokens < 0 || tokens > INT_MAX - 256 || prompts < 0) return B2G_ESHAPE;
-  if (tokens == 0 || prompts == 0) return B2G_OK;
-  const int rc = check_serving_attention(heads_q, heads_k, head_dim, dtype, sm_scale, strides, 8,
-                                         {q, k, v, o});
-  if (rc != B2G_OK) return rc;
-  if (cu_seqlens == nullptr) return B2G_EINVAL;
-  if (reinterpret_cast<uintptr_t>(lse) % alignof(float) != 0) return B2G_EALIGN;
-  const int64_t blocks = packed_blocks(prompts, tokens);
-  if (blocks * heads_q > INT_MAX) return B2G_ESHAPE;
-  const int sms = current_device_sms();
-  if (sms <= 0) return B2G_ENODEVICE;
-  if (workspace == nullptr || workspace_bytes < packed_workspace(prompts, tokens, sms))
-    return B2G_EWORKSPACE;
-  if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return B2G_EALIGN;
-
-  FmhaParams prm;
-  std::memset(&prm, 0, sizeof(prm));
-  // (token, head) strides as a batch of one: (batch, head, sequence, dim)
-  auto encode = [&](CUtensorMap* map, const void* base, int heads, const int64_t* st) {
-    const int64_t four[4] = {st[0] * tokens, st[1], st[0], 1};
-    return encode_bshd_view(map, base, dtype, head_dim, static_cast<int>(tokens), heads, 1, four);
-  };
-  if (!encode(&prm.tmQ, q, heads_q, strides) || !encode(&prm.tmK, k, heads_k, strides + 2) ||
-      !encode(&prm.tmV, v, heads_k, strides + 4))
-    return B2G_ETENSORMAP;
-  uint8_t* ws = static_cast<uint8_t*>(workspace) + workspace_flag_bytes(sms);
-  PackedPlanParams pl;
-  pl.cu = cu_seqlens;
-  pl.count = reinterpret_cast<int32_t*>(ws);
-  pl.plan = reinterpret_cast<int4*>(ws + 256);
-  pl.status = status;
-  pl.prompts = prompts;
-  pl.tokens = static_cast<int32_t>(tokens);
-  pl.capacity = static_cast<int32_t>(blocks);
-  prm.plan = pl.plan;
-  prm.plan_count = pl.count;
-  prm.O = o;
-  prm.o_ss = strides[6];
-  prm.o_sh = strides[7];
-  prm.V = v;
-  prm.v_ss = strides[4];
-  prm.v_sh = strides[5];
-  prm.lse = lse;
-  prm.status = status;
-  prm.B = 1;
-  prm.HQ = heads_q;
-  prm.HK = heads_k;
-  prm.S_q = prm.S_k = static_cast<int32_t>(tokens);
-  prm.scale_log2 = sm_scale * 1.4426950408889634f;
-  prm.timeout_ns = wait_timeout_ns();
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  packed_plan_kernel<<<1, kPlanThreads, 0, s>>>(pl);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return static_cast<int>(e);
-  const bool bf16 = dtype == B2G_DT_BF16;
-  if (head_dim == 128)
-    return bf16 ? launch_fmha<128, true, true>(prm, blocks * heads_q, s)
-                : launch_fmha<128, false, true>(prm, blocks * heads_q, s);
-  return bf16 ? launch_fmha<64, true, true>(prm, blocks * heads_q, s)
-              : launch_fmha<64, false, true>(prm, blocks * heads_q, s);
+    return bf16 ? launch_fmha<128, true>(prm, batch, heads_q, seqlen_q, s)
+                : launch_fmha<128, false>(prm, batch, heads_q, seqlen_q, s);
+  return bf16 ? launch_fmha<64, true>(prm, batch, heads_q, seqlen_q, s)
+              : launch_fmha<64, false>(prm, batch, heads_q, seqlen_q, s);
 }
 
 // Evaluates the FMHA's FMA-pipe exponential on caller data: y_scalar[i] =

@@ -363,113 +363,6 @@ __device__ __noinline__ void add_odd_cache_values(const TreeParams& p, const Seg
   }
 }
 
-// One tile's softmax for a thread's row: NCH chunks of 32 score columns from
-// chunk c0 on, weights for those and zeros for the others into P. Keeps the
-// running maximum (log2 units) and sum.
-template <int D, bool kBF16, int NCH>
-__device__ __forceinline__ void tree_softmax(uint32_t s_col, uint32_t o_col, uint32_t c0, float sl2,
-                                             bool masked, const uint32_t (&seen)[4], bool first,
-                                             float& m_run, float& l_run, uint32_t p_bar0,
-                                             uint32_t p_bar1, uint32_t lane) {
-  constexpr int kRegs = NCH == 4 ? 4 : NCH;
-  uint32_t s[32 * kRegs];
-#pragma unroll
-  for (int c = 0; c < NCH; ++c)
-    tmem_ld_32x32b_x32(s_col + 32u * (c0 + c), *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
-  tmem_wait_ld();
-  if (masked) {
-#pragma unroll
-    for (int c = 0; c < NCH; ++c)
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (!((seen[c] >> i) & 1u)) s[32 * c + i] = __float_as_uint(-INFINITY);
-  }
-  float m8[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m8[i] = fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 8]));
-#pragma unroll
-  for (int c = 16; c < 32 * NCH; c += 16)
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      m8[i] = fmax3(m8[i], __uint_as_float(s[c + i]), __uint_as_float(s[c + 8 + i]));
-  const float mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]),
-                         fmaxf(m8[6], m8[7]));
-  constexpr float kRescaleLog2 = 8.0f;  // see attention.cu
-  const float m_cand = mx * sl2;
-  const bool move = m_cand > m_run + kRescaleLog2;
-  const float m_new = move ? m_cand : m_run;
-  float alpha = 1.0f;
-  if (move) alpha = poly_exp2(m_run - m_new);
-  if (!first && __any_sync(0xffffffffu, move)) {
-#pragma unroll 1
-    for (uint32_t d = 0; d < static_cast<uint32_t>(D); d += 16u) {
-      uint32_t o[16];
-      tmem_ld_32x32b_x16(o_col + d, o);
-      tmem_wait_ld();
-#pragma unroll
-      for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
-      tmem_st_32x32b_x16(o_col + d, o);
-    }
-  }
-  const float off = m_new == -INFINITY ? 0.0f : -m_new;
-  const float2 sl2x2 = make_float2(sl2, sl2), negm = make_float2(off, off);
-  float2 acc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
-                   make_float2(0.f, 0.f)};
-  uint32_t buf[2][32];
-  if constexpr (NCH == 4) tmem_ld_32x32b_x32(s_col + 64u, buf[0]);
-  if constexpr (NCH < 4) {
-    uint32_t zero[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) zero[i] = 0u;
-#pragma unroll
-    for (uint32_t c = 0; c < 4; ++c)
-      if (c < c0 || c >= c0 + NCH) tmem_st_32x32b_x16(s_col + 16u * c, zero);
-  }
-#pragma unroll
-  for (int c = 0; c < NCH; ++c) {
-    if (NCH == 4 && c == 2) {
-      tmem_wait_ld();
-      regs_ready(buf[0]);
-      tmem_ld_32x32b_x32(s_col + 96u, buf[1]);
-    }
-    if (NCH == 4 && c == 3) {
-      tmem_wait_ld();
-      regs_ready(buf[1]);
-    }
-    uint32_t cur[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) cur[i] = c < 2 ? s[32 * c + i] : buf[c & 1][i];
-    if (c >= 2 && masked) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (!((seen[c] >> i) & 1u)) cur[i] = __float_as_uint(-INFINITY);
-    }
-    uint32_t pk[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float2 x = __ffma2_rn(
-          make_float2(__uint_as_float(cur[2 * i]), __uint_as_float(cur[2 * i + 1])), sl2x2, negm);
-      const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-      acc[i & 3] = __fadd2_rn(acc[i & 3], e);
-      pk[i] = pack2<kBF16>(e.x, e.y);
-    }
-    tmem_st_32x32b_x16(s_col + 16u * (c0 + static_cast<uint32_t>(c)), pk);
-    if (c + 1 == NCH || (NCH == 4 && c == 1)) {
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (c == 1 || NCH < 4) mbar_arrive(p_bar0);
-        if (c + 1 == NCH) mbar_arrive(p_bar1);
-      }
-    }
-  }
-  const float2 a01 = __fadd2_rn(acc[0], acc[1]), a23 = __fadd2_rn(acc[2], acc[3]);
-  const float2 a = __fadd2_rn(a01, a23);
-  l_run = fmaf(l_run, alpha, a.x + a.y);
-  m_run = m_new;
-}
-
 // Joins share k of a block: a lane to a row, E float4 columns by P parts at a time,
 // whose loads are all in flight together (with eight warps on the SM their latency
 // and that of the arithmetic between them is what bounds this, so what depends on
@@ -861,13 +754,13 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
               seen[c] = seen_bits(p, w.e, tok, kb + 32 * static_cast<int32_t>(c0 + c));
         }
         if (per == 4u)
-          tree_softmax<D, kBF16, 4>(s_col, o_col, 0u, p.scale_log2, masked, seen, first, m_run,
+          tile_softmax<D, kBF16, 4>(s_col, o_col, 0u, p.scale_log2, masked, seen, first, m_run,
                                     l_run, p_full(t, 0), p_full(t, 1), lane);
         else if (per == 2u)
-          tree_softmax<D, kBF16, 2>(s_col, o_col, c0, p.scale_log2, masked, seen, first, m_run,
+          tile_softmax<D, kBF16, 2>(s_col, o_col, c0, p.scale_log2, masked, seen, first, m_run,
                                     l_run, p_full(t, 0), p_full(t, 1), lane);
         else
-          tree_softmax<D, kBF16, 1>(s_col, o_col, c0, p.scale_log2, masked, seen, first, m_run,
+          tile_softmax<D, kBF16, 1>(s_col, o_col, c0, p.scale_log2, masked, seen, first, m_run,
                                     l_run, p_full(t, 0), p_full(t, 1), lane);
       }
 

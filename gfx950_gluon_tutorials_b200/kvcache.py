@@ -27,6 +27,7 @@ from .ops import _require_cuda, _stream_handle, status_tensor
 
 _DT = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
 MAX_REQUESTS = 8192
+_I64x10 = ctypes.c_int64 * 10
 
 
 class StepMaps(NamedTuple):
@@ -41,7 +42,8 @@ class StepMaps(NamedTuple):
 
 
 def _int_vector(t: torch.Tensor, n: int | None, dtype: torch.dtype, name: str) -> torch.Tensor:
-    if t.dtype != dtype or t.dim() != 1 or (n is not None and t.shape[0] != n):
+    shape = t.shape
+    if t.dtype is not dtype or len(shape) != 1 or (n is not None and shape[0] != n):
         want = "" if n is None else f"{n} "
         raise ValueError(f"{name} must be a 1-D tensor of {want}{dtype}, got {tuple(t.shape)} {t.dtype}")
     return t if t.is_contiguous() else t.contiguous()
@@ -67,7 +69,8 @@ def map_step(cached_lens: torch.Tensor, new_lens: torch.Tensor, page_counts: tor
     if block_tables.dim() != 2 or block_tables.dtype != torch.int32:
         raise ValueError("block_tables must be a 2-D int32 tensor")
     requests, max_pages = block_tables.shape
-    if max_pages > 1 and block_tables.stride(1) != 1:
+    table_stride, column_stride = block_tables.stride()
+    if max_pages > 1 and column_stride != 1:
         raise ValueError("block_tables is updated in place: its rows must be contiguous")
     cached_lens = _int_vector(cached_lens, requests, torch.int32, "cached_lens")
     new_lens = _int_vector(new_lens, requests, torch.int32, "new_lens")
@@ -85,7 +88,7 @@ def map_step(cached_lens: torch.Tensor, new_lens: torch.Tensor, page_counts: tor
     base = ints.data_ptr()
     rc = _lib.lib().b2g_kv_map_step(
         cached_lens.data_ptr(), new_lens.data_ptr(), page_counts.data_ptr(),
-        block_tables.data_ptr(), block_tables.stride(0), requests, max_pages,
+        block_tables.data_ptr(), table_stride, requests, max_pages,
         free_pages.data_ptr(), free_pages.shape[0], num_free.data_ptr(), page_size, n,
         slots.data_ptr(), base, base + 4 * n, base + 4 * (n + requests + 1),
         base + 4 * (n + 2 * requests + 1), base + 4 * (n + 3 * requests + 1),
@@ -127,8 +130,8 @@ def write_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: t
         k = k.contiguous()
     if v.stride(2) != 1:
         v = v.contiguous()
-    strides = (ctypes.c_int64 * 10)(*k.stride()[:2], *v.stride()[:2], *k_cache.stride()[:3],
-                                    *v_cache.stride()[:3])
+    strides = _I64x10(*k.stride()[:2], *v.stride()[:2], *k_cache.stride()[:3],
+                      *v_cache.stride()[:3])
     rc = _lib.lib().b2g_kv_write(
         k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), strides,
         slots.data_ptr(), tokens, heads, dim, pages, page, _DT[k.dtype],

@@ -25,7 +25,13 @@ _workspaces: dict[tuple[int, int], torch.Tensor] = {}
 _status: dict[int, torch.Tensor] = {}
 
 
+# the current stream's handle without a Stream object around it: 0.1 us against 2.2
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream_handle(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -47,6 +53,9 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     The kernels leave it zeroed after a successful run, so it is reused as is.
     """
     key = (device.index, _stream_handle(device))
+    ws = _workspaces.get(key)
+    if ws is not None and ws.numel() >= nbytes:
+        return ws
     with _ws_lock:
         ws = _workspaces.get(key)
         if ws is None or ws.numel() < nbytes:
@@ -57,6 +66,9 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
 
 def status_tensor(device: torch.device) -> torch.Tensor:
     """The device status word that kernels on ``device`` report bounded-wait timeouts in."""
+    st = _status.get(device.index)
+    if st is not None:
+        return st
     with _ws_lock:
         st = _status.get(device.index)
         if st is None:
