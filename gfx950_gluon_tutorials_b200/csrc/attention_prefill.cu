@@ -205,26 +205,23 @@ struct PrefillItem {
 
 // Walks a CTA's items; the plan's entry of the next one is loaded an item ahead.
 struct PrefillWalk {
-  int32_t item, items, row_items, pairs;
+  int32_t item, items, row_blocks, row_items, pairs;
   uint32_t turn;
   int4 ahead;
 
   __device__ __forceinline__ void begin(const PrefillParams& p) {
     const int2 c = *p.counts;
     pairs = (p.HQ + 1) / 2;
+    row_blocks = c.x;
     row_items = c.x * p.HQ;
     items = row_items + c.y * pairs;
     item = static_cast<int32_t>(blockIdx.x);
     turn = 0;
     fetch(p);
   }
-  __device__ __forceinline__ int32_t entry() const {
-    return item < row_items ? item / heads() : row_items / heads() + (item - row_items) / pairs;
-  }
-  __device__ __forceinline__ int32_t heads() const { return hq; }
   __device__ __forceinline__ void fetch(const PrefillParams& p) {
-    hq = p.HQ;
-    if (item < items) ahead = p.plan[entry()];
+    if (item < items)
+      ahead = p.plan[item < row_items ? item / p.HQ : row_blocks + (item - row_items) / pairs];
   }
   __device__ __forceinline__ bool next(const PrefillParams& p, PrefillItem& w) {
     if (item >= items) return false;
@@ -249,8 +246,6 @@ struct PrefillWalk {
     fetch(p);
     return true;
   }
-
-  int32_t hq;
 };
 
 template <int D, bool kBF16>
@@ -263,7 +258,7 @@ __global__ void __launch_bounds__(PrefillPlan<D>::kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   const uint32_t sbase = smem_u32(smem);
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
   const uint32_t bar0 = sbase + PP::kBarOff;
   const uint32_t q_full = bar0, q_empty = bar0 + 8u;  // q_empty: the item's last S is done with Q
@@ -372,92 +367,100 @@ __global__ void __launch_bounds__(PrefillPlan<D>::kThreads, 1)
     // ----------------------------------------------------------- MMA issue --
     // Per slot the order is S_0, PV_0, S_1, PV_1, ... (P lies in S's columns, and
     // one thread's MMAs run in issue order); the slots take turns, so one's softmax
-    // runs during the other's products.
-    if (lane == 0) {
+    // runs during the other's products. The whole warp runs this and one lane issues
+    // (see elect_one), what is there long before P is waited for before it, and
+    // descriptors are sums: with a single-thread branch the issue took longer than the
+    // products (12031 tokens x 32 heads: 1124 us then, 945-963 so).
+    {
       constexpr uint32_t idesc_s = fmha_idesc_s<D, kBF16>();
       constexpr uint32_t idesc_pv = fmha_idesc_pv<D, kBF16>();
       uint32_t last_bar = 0, last_par = 0;  // the newest commit: all earlier MMAs precede it
       uint32_t base = 0, ic = 0;            // ring stages before the item, items
-      uint32_t steps[2] = {0u, 0u};         // tiles of each slot (phases of s_full, p_full)
-      uint32_t titems[2] = {0u, 0u};        // items of each slot (phases of o_done, o_free)
+      uint32_t steps0 = 0, steps1 = 0;      // tiles of each slot (phases of s_full, p_full)
+      uint32_t items0 = 0, items1 = 0;      // items of each slot (phases of o_done, o_free)
       bool alive = true;
-      while (alive && walk.next(p, w)) {
-        auto ready = [&](uint32_t bar, uint32_t st) {
-          return fmha_wait(bar, (st / KS) & 1u, abort_flag, p, B2G_SITE_FULL);
-        };
-        // S of slot t's tile j, whose K has to be there
-        auto issue_s = [&](uint32_t t, int32_t j) {
-          const uint32_t s = (base + w.stage(t, j)) % KS;
-          const uint32_t k_base = sbase + PP::kKOff + s * PP::kTile;
-          const uint32_t q_base = sbase + PP::kQOff + t * PP::kTile;
+      auto wait = [&](uint32_t bar, uint32_t parity, int site) {
+        return __all_sync(0xffffffffu, fmha_wait(bar, parity & 1u, abort_flag, p, site)) != 0;
+      };
+      auto commit = [&](uint32_t bar) {
+        if (elect_one()) tc_commit<1>(bar);
+      };
+      const uint64_t q_desc = sdesc_kmajor_sw128(sbase + PP::kQOff);
+      const uint64_t k_desc = sdesc_kmajor_sw128(sbase + PP::kKOff);
+      const uint64_t v_desc = sdesc_mnmajor_sw128(sbase + PP::kVOff, kSlabBytes, 1024u);
+      // S of slot t with the K tile of stage s
+      auto issue_s = [&](uint32_t t, uint32_t s) {
+        const uint64_t qd = q_desc + t * (PP::kTile >> 4), kd = k_desc + s * (PP::kTile >> 4);
 #pragma unroll
-          for (uint32_t kk = 0; kk < D / 16; ++kk) {
-            const uint64_t ad = sdesc_kmajor_sw128(q_base + (kk >> 2) * kSlabBytes) + 2u * (kk & 3u);
-            const uint64_t bd = sdesc_kmajor_sw128(k_base + (kk >> 2) * kSlabBytes) + 2u * (kk & 3u);
-            mma_f16<1>(tmem_base + PP::kS + t * PP::kTileCols, ad, bd, idesc_s, kk > 0 ? 1u : 0u);
-          }
-          tc_commit<1>(s_full(t));
-          last_bar = s_full(t);
-          last_par = steps[t] & 1u;
-          if (!w.shared || t + 1u == w.slots) tc_commit<1>(k_empty(s));
-          if (j + 1 == w.n && t + 1u == w.slots) tc_commit<1>(q_empty);
-        };
-        if (!fmha_wait(q_full, ic & 1u, abort_flag, p, B2G_SITE_FULL)) break;
+        for (uint32_t kk = 0; kk < D / 16; ++kk) {
+          const uint32_t at = (kk >> 2) * (kSlabBytes >> 4) + 2u * (kk & 3u);
+          if (elect_one())
+            mma_f16<1>(tmem_base + PP::kS + t * PP::kTileCols, qd + at, kd + at, idesc_s,
+                       kk > 0 ? 1u : 0u);
+        }
+        commit(s_full(t));
+      };
+      while (alive && walk.next(p, w)) {
+        w.n = uniform(w.n);
+        w.slots = uniform(w.slots);
+        w.shared = uniform(static_cast<int32_t>(w.shared)) != 0;
+        w.by_rows = uniform(static_cast<int32_t>(w.by_rows)) != 0;
+        const uint32_t dual = w.shared ? 0u : 1u;
+        if (!wait(q_full, ic, B2G_SITE_FULL)) break;
         for (uint32_t t = 0; t < w.slots; ++t) {
-          const uint32_t st = base + w.stage(t, 0);
-          if (!ready(k_full(st % KS), st)) {
+          const uint32_t st = base + dual * t, s = st % KS;
+          if (!wait(k_full(s), st / KS, B2G_SITE_FULL)) {
             alive = false;
             break;
           }
           tc_fence_after();
-          issue_s(t, 0);
+          issue_s(t, s);
+          if (dual || t + 1u == w.slots) commit(k_empty(s));
         }
-        for (int32_t j = 0; alive && j < w.n; ++j) {
-          for (uint32_t t = 0; alive && t < w.slots; ++t) {
-            const int32_t n = w.tiles(t);
-            if (j >= n) continue;
-            const uint32_t st = base + w.stage(t, j), s = st % KS;
-            if (!ready(v_full(s), st) ||
-                // the previous item's epilogue must have read this slot's O
-                (j == 0 && titems[t] > 0 &&
-                 !fmha_wait(o_free(t), (titems[t] - 1u) & 1u, abort_flag, p, B2G_SITE_ACC_EMPTY))) {
-              alive = false;
-              break;
-            }
-            const uint32_t v_base = sbase + PP::kVOff + s * PP::kTile;
-            const uint32_t p_col = tmem_base + PP::kS + t * PP::kTileCols;
-            for (uint32_t half = 0; half < 2; ++half) {
-              if (!fmha_wait(p_full(t, half), steps[t] & 1u, abort_flag, p, B2G_SITE_ACC_FULL)) {
-                alive = false;
-                break;
-              }
-              tc_fence_after();
+        if (w.n == 1) commit(q_empty);
+        // slot t's step j: PV of its tile, then S of its next one
+        auto slot_step = [&](uint32_t t, int32_t j, uint32_t& steps, uint32_t& items) {
+          const int32_t n = w.tiles(t);
+          if (j >= n) return true;
+          const uint32_t st = base + (static_cast<uint32_t>(j) << dual) + dual * t, s = st % KS;
+          const uint32_t st1 = st + 1u + dual, s1 = st1 % KS;
+          const bool more = j + 1 < n, last = dual || t + 1u == w.slots;
+          if (!wait(v_full(s), st / KS, B2G_SITE_FULL)) return false;
+          if (more && !wait(k_full(s1), st1 / KS, B2G_SITE_FULL)) return false;
+          if (j == 0 && items > 0 && !wait(o_free(t), items - 1u, B2G_SITE_ACC_EMPTY)) return false;
+          const uint64_t vd = v_desc + s * (PP::kTile >> 4);
+          const uint32_t p_col = tmem_base + PP::kS + t * PP::kTileCols;
 #pragma unroll
-              for (uint32_t k4 = 0; k4 < 4; ++k4) {
-                const uint32_t kk = half * 4u + k4;
-                const uint64_t bd = sdesc_mnmajor_sw128(v_base + kk * 2048u, kSlabBytes, 1024u);
-                mma_f16_ts(tmem_base + PP::kO + t * PP::kTileCols, p_col + kk * 8u, bd, idesc_pv,
-                           (j > 0 || kk > 0) ? 1u : 0u);
-              }
+          for (uint32_t half = 0; half < 2; ++half) {
+            if (!wait(p_full(t, half), steps, B2G_SITE_ACC_FULL)) return false;
+            tc_fence_after();
+#pragma unroll
+            for (uint32_t k4 = 0; k4 < 4; ++k4) {
+              const uint32_t kk = half * 4u + k4;
+              if (elect_one())
+                mma_f16_ts(tmem_base + PP::kO + t * PP::kTileCols, p_col + kk * 8u,
+                           vd + kk * (2048u >> 4), idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
             }
-            if (!alive) break;
-            ++steps[t];
-            if (j + 1 == n) {
-              tc_commit<1>(o_done(t));
-              last_bar = o_done(t);
-              last_par = titems[t] & 1u;
-              ++titems[t];
-            } else {
-              const uint32_t next = base + w.stage(t, j + 1);
-              if (!ready(k_full(next % KS), next)) {
-                alive = false;
-                break;
-              }
-              tc_fence_after();
-              issue_s(t, j + 1);
-            }
-            if (!w.shared || t + 1u == w.slots) tc_commit<1>(v_empty(s));
           }
+          ++steps;
+          if (more) {
+            issue_s(t, s1);
+            last_bar = s_full(t);
+            last_par = steps & 1u;
+            if (last) commit(k_empty(s1));
+          } else {
+            commit(o_done(t));
+            last_bar = o_done(t);
+            last_par = items & 1u;
+            ++items;
+          }
+          if (last) commit(v_empty(s));
+          return true;
+        };
+        for (int32_t j = 0; alive && j < w.n; ++j) {
+          alive = slot_step(0u, j, steps0, items0) &&
+                  (w.slots == 1u || slot_step(1u, j, steps1, items1));
+          if (j + 2 == w.n) commit(q_empty);  // the item's last S is issued
         }
         base += w.stages();
         ++ic;

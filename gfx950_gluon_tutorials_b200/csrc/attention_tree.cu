@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
     return;
   }
   const uint32_t sbase = smem_u32(smem);
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
   const uint32_t bar0 = sbase + TP::kBarOff;
   const uint32_t q_full = bar0, q_empty = bar0 + 8u;
@@ -559,103 +559,105 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
     }
   } else if (warp == 1) {
     // ----------------------------------------------------------- MMA issue --
-    if (lane == 0) {
+    // The whole warp runs this and one lane issues; see attention_prefill.cu.
+    {
       constexpr uint32_t idesc_s = fmha_idesc_s<D, kBF16>();
       constexpr uint32_t idesc_pv = fmha_idesc_pv<D, kBF16>();
       uint32_t last_bar = 0, last_par = 0;  // the newest commit: all earlier MMAs precede it
       uint32_t base = 0, ic = 0;            // ring loads before the segment, segments
-      uint32_t steps[2] = {0u, 0u};         // tiles of each warpgroup (phases of s_full, p_full)
-      uint32_t titems[2] = {0u, 0u};        // segments of each (phases of o_done, o_free)
+      uint32_t steps0 = 0, steps1 = 0;      // tiles of each warpgroup (phases of s_full, p_full)
+      uint32_t items0 = 0, items1 = 0;      // segments of each (phases of o_done, o_free)
       bool alive = true;
+      auto wait = [&](uint32_t bar, uint32_t parity, int site) {
+        return __all_sync(0xffffffffu, fmha_wait(bar, parity & 1u, abort_flag, p, site)) != 0;
+      };
+      auto commit = [&](uint32_t bar) {
+        if (elect_one()) tc_commit<1>(bar);
+      };
+      const uint64_t q_desc = sdesc_kmajor_sw128(sbase + TP::kQOff);
+      const uint64_t k_desc = sdesc_kmajor_sw128(sbase + TP::kRingOff);
+      const uint64_t v_desc = sdesc_mnmajor_sw128(sbase + TP::kRingOff, kSlabBytes, 1024u);
       while (alive && walk.next(p, w)) {
-        const int32_t n = w.j1 - w.j0;
-        auto k_load = [&](int32_t j) { return base + k_order(w.two, j); };
-        auto ready = [&](uint32_t load) {
-          return fmha_wait(full(load % NS), (load / NS) & 1u, abort_flag, p, B2G_SITE_FULL);
-        };
-        // S = Q K^T of step j for warpgroup t
-        auto issue_s = [&](uint32_t t, int32_t j) {
-          const uint32_t k_base = sbase + TP::kRingOff + (k_load(j) % NS) * TP::kTile;
-          const uint32_t q_base = sbase + TP::kQOff + (w.two ? t * TP::kTile : 0u);
+        const int32_t n = uniform(w.j1 - w.j0);
+        const bool two = uniform(static_cast<int32_t>(w.two)) != 0;
+        const uint32_t slots = two || n > 1 ? 2u : 1u;
+        // S = Q K^T of tile j for warpgroup t
+        auto issue_s = [&](uint32_t t, int32_t j, uint32_t s) {
+          const uint64_t qd = q_desc + (two ? t * (TP::kTile >> 4) : 0u);
+          const uint64_t kd = k_desc + s * (TP::kTile >> 4);
 #pragma unroll
           for (uint32_t kk = 0; kk < D / 16; ++kk) {
-            const uint64_t ad = sdesc_kmajor_sw128(q_base + (kk >> 2) * kSlabBytes) + 2u * (kk & 3u);
-            const uint64_t bd = sdesc_kmajor_sw128(k_base + (kk >> 2) * kSlabBytes) + 2u * (kk & 3u);
-            mma_f16<1>(tmem_base + TP::kS + t * TP::kTileCols, ad, bd, idesc_s, kk > 0 ? 1u : 0u);
+            const uint32_t at = (kk >> 2) * (kSlabBytes >> 4) + 2u * (kk & 3u);
+            if (elect_one())
+              mma_f16<1>(tmem_base + TP::kS + t * TP::kTileCols, qd + at, kd + at, idesc_s,
+                         kk > 0 ? 1u : 0u);
           }
-          tc_commit<1>(s_full(t));
-          last_bar = s_full(t);
-          last_par = steps[t] & 1u;
+          commit(s_full(t));
           // the tile of K is free after its last product, Q after the block's
-          if (!w.two || t == 1u) {
-            tc_commit<1>(empty(k_load(j) % NS));
-            if (j + 1 == n) tc_commit<1>(q_empty);
+          if (!two || t == 1u) {
+            commit(empty(s));
+            if (j + 1 == n) commit(q_empty);
           }
         };
-        if (!fmha_wait(q_full, ic & 1u, abort_flag, p, B2G_SITE_FULL)) break;
-        for (uint32_t t = 0; t < w.slots; ++t) {
-          const int32_t j = w.two ? 0 : static_cast<int32_t>(t);
-          if (!ready(k_load(j))) {
+        if (!wait(q_full, ic, B2G_SITE_FULL)) break;
+        for (uint32_t t = 0; t < slots; ++t) {
+          const int32_t j = two ? 0 : static_cast<int32_t>(t);
+          const uint32_t ld = base + k_order(two, j);
+          if (!wait(full(ld % NS), ld / NS, B2G_SITE_FULL)) {
             alive = false;
             break;
           }
           tc_fence_after();
-          issue_s(t, j);
+          issue_s(t, j, ld % NS);
         }
-        for (int32_t j = 0; alive && j < n; ++j) {
-          const uint32_t v_load = base + v_order(w.two, j, n);
-          if (!ready(v_load)) {
-            alive = false;
-            break;
-          }
-          const uint32_t v_base = sbase + TP::kRingOff + (v_load % NS) * TP::kTile;
-          const uint32_t t_begin = w.two ? 0u : static_cast<uint32_t>(j) & 1u;
-          const uint32_t t_end = w.two ? 2u : t_begin + 1u;
-          const int32_t next = j + (w.two ? 1 : 2);
-          const bool first = w.two ? j == 0 : j < 2;
-          for (uint32_t t = t_begin; alive && t < t_end; ++t) {
-            const uint32_t p_col = tmem_base + TP::kS + t * TP::kTileCols;
-            if (first && titems[t] > 0 &&
-                !fmha_wait(o_free(t), (titems[t] - 1u) & 1u, abort_flag, p, B2G_SITE_ACC_EMPTY)) {
-              alive = false;
-              break;
-            }
-            for (uint32_t half = 0; half < 2; ++half) {
-              if (!fmha_wait(p_full(t, half), steps[t] & 1u, abort_flag, p, B2G_SITE_ACC_FULL)) {
-                alive = false;
-                break;
-              }
-              tc_fence_after();
+        // warpgroup t's PV of tile j, then S of its next one
+        auto slot_step = [&](uint32_t t, int32_t j, uint32_t& steps, uint32_t& items) {
+          const int32_t next = j + (two ? 1 : 2);
+          const bool first = two ? j == 0 : j < 2, more = next < n;
+          const uint32_t lv = base + v_order(two, j, n), lk = base + k_order(two, next);
+          if (!wait(full(lv % NS), lv / NS, B2G_SITE_FULL)) return false;
+          // with a row tile to each warpgroup K of the next tile is there by now
+          if (two && more && !wait(full(lk % NS), lk / NS, B2G_SITE_FULL)) return false;
+          if (first && items > 0 && !wait(o_free(t), items - 1u, B2G_SITE_ACC_EMPTY)) return false;
+          const uint64_t vd = v_desc + (lv % NS) * (TP::kTile >> 4);
+          const uint32_t p_col = tmem_base + TP::kS + t * TP::kTileCols;
 #pragma unroll
-              for (uint32_t k4 = 0; k4 < 4; ++k4) {
-                const uint32_t kk = half * 4u + k4;
-                const uint64_t bd = sdesc_mnmajor_sw128(v_base + kk * 2048u, kSlabBytes, 1024u);
-                mma_f16_ts(tmem_base + TP::kO + t * TP::kTileCols, p_col + kk * 8u, bd, idesc_pv,
-                           (!first || kk > 0) ? 1u : 0u);
-              }
-            }
-            if (!alive) break;
-            ++steps[t];
-            if (next >= n) {
-              tc_commit<1>(o_done(t));
-              last_bar = o_done(t);
-              last_par = titems[t] & 1u;
-              ++titems[t];
-              continue;
-            }
-            if (!ready(k_load(next))) {
-              alive = false;
-              break;
-            }
+          for (uint32_t half = 0; half < 2; ++half) {
+            if (!wait(p_full(t, half), steps, B2G_SITE_ACC_FULL)) return false;
             tc_fence_after();
-            issue_s(t, next);
+#pragma unroll
+            for (uint32_t k4 = 0; k4 < 4; ++k4) {
+              const uint32_t kk = half * 4u + k4;
+              if (elect_one())
+                mma_f16_ts(tmem_base + TP::kO + t * TP::kTileCols, p_col + kk * 8u,
+                           vd + kk * (2048u >> 4), idesc_pv, (!first || kk > 0) ? 1u : 0u);
+            }
           }
-          if (alive) tc_commit<1>(empty(v_load % NS));
+          ++steps;
+          if (!two) commit(empty(lv % NS));
+          if (more) {
+            if (!two && !wait(full(lk % NS), lk / NS, B2G_SITE_FULL)) return false;
+            tc_fence_after();
+            issue_s(t, next, lk % NS);
+            last_bar = s_full(t);
+            last_par = steps & 1u;
+          } else {
+            commit(o_done(t));
+            last_bar = o_done(t);
+            last_par = items & 1u;
+            ++items;
+          }
+          if (two && t == 1u) commit(empty(lv % NS));
+          return true;
+        };
+        for (int32_t j = 0; alive && j < n; ++j) {
+          if (two || (j & 1) == 0) alive = slot_step(0u, j, steps0, items0);
+          if (alive && (two || (j & 1) != 0)) alive = slot_step(1u, j, steps1, items1);
         }
         base += 2u * static_cast<uint32_t>(n);
         ++ic;
       }
-      // all MMAs issued by this thread finish before TMEM can be freed
+      // all MMAs issued by this warp finish before TMEM can be freed
       if (last_bar != 0u) {
         uint32_t spins = 0;
         while (!mbar_try_wait(last_bar, last_par) && spins < (1u << 22)) ++spins;
