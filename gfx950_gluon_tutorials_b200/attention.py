@@ -174,45 +174,55 @@ def run_gluon_attention(q, k, v, o, metadata: MetaData, scale_on_q: bool = True)
     return attention_fwd(q, k, v, o, sm_scale=metadata.sm_scale, layout=metadata.layout)
 
 
-def _packed(t: torch.Tensor) -> bool:
-    """Whether a (tokens, heads, dim) tensor can be read or written where it lies: unit
-    dim stride, 16-byte aligned base and rows."""
+def _packed(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
+    """A (tokens, heads, dim) tensor and its token and head strides, copied unless it can be
+    read where it lies: unit dim stride, 16-byte aligned base and rows."""
     s0, s1, s2 = t.stride()
-    return s2 == 1 and s0 > 0 < s1 and not ((s0 | s1) & 7 or t.data_ptr() & 15)
+    if s2 == 1 and s0 > 0 < s1 and not ((s0 | s1) & 7 or t.data_ptr() & 15):
+        return t, s0, s1
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride(0), t.stride(1)
 
 
-def _readable(t: torch.Tensor) -> torch.Tensor:
-    return t if _packed(t) else t.clone(memory_format=torch.contiguous_format)
+def _check_packed(q: torch.Tensor, hk: int, o, lse) -> tuple:
+    """(tokens, HQ, D, the code of q's dtype) of valid packed queries with their o and lse."""
+    dtype = _DT.get(q.dtype)
+    if dtype is None:
+        raise ValueError("q must be float16 or bfloat16")
+    shape = q.shape
+    if len(shape) != 3:
+        raise ValueError("q must be (tokens, heads, head_dim)")
+    tokens, hq, dim = shape
+    if dim not in HEAD_DIMS:
+        raise ValueError(f"head dim must be one of {HEAD_DIMS}, got {dim}")
+    if hk < 1 or hq % hk:
+        raise ValueError("query heads must be a multiple of key/value heads")
+    if o is not None and (o.shape != shape or o.dtype is not q.dtype):
+        raise ValueError("o must have q's shape and dtype")
+    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (hq, tokens)
+                            or not lse.is_contiguous()):
+        raise ValueError(f"lse must be a contiguous float32 ({hq}, {tokens}) tensor")
+    return tokens, hq, dim, dtype
 
 
-def _with_workspace(call, args: tuple, dev: torch.device, nbytes) -> int:
-    """``call(*args, workspace, its size, status, stream)`` with the stream's workspace as it
-    is; asks how large it has to be only when the call finds it too small."""
+def _run_packed(call, nbytes, dev, q, o, lse, args) -> torch.Tensor:
+    """``call(*args(out, its strides, lse), workspace, its size, status, stream)`` into o (a new
+    tensor if it is None) with the stream's workspace as it is; asks ``nbytes`` how large that has
+    to be only when the call finds it too small."""
+    if o is None:
+        o = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    out, o_token, o_head = _packed(o)  # a copy keeps the rows past the last sequence
+    args = args(out.data_ptr(), o_token, o_head, None if lse is None else lse.data_ptr())
     ws, status, stream = workspace(0, dev), status_tensor(dev).data_ptr(), _stream_handle(dev)
     rc = call(*args, ws.data_ptr(), ws.numel(), status, stream)
     if rc == _lib.EWORKSPACE:
         ws = workspace(nbytes(), dev)
         rc = call(*args, ws.data_ptr(), ws.numel(), status, stream)
-    return rc
-
-
-def _check_packed(q: torch.Tensor, hk: int, o, lse) -> tuple[int, int, int, torch.Tensor]:
-    """Shapes of q, its output and its lse; returns (tokens, heads, dim, o)."""
-    if q.dtype not in _DT:
-        raise ValueError("q must be float16 or bfloat16")
-    tokens, hq, dim = q.shape
-    if dim not in HEAD_DIMS:
-        raise ValueError(f"head dim must be one of {HEAD_DIMS}, got {dim}")
-    if hk < 1 or hq % hk:
-        raise ValueError("query heads must be a multiple of key/value heads")
-    if o is None:
-        o = torch.empty((tokens, hq, dim), dtype=q.dtype, device=q.device)
-    elif o.shape != q.shape or o.dtype != q.dtype:
-        raise ValueError("o must have q's shape and dtype")
-    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (hq, tokens)
-                            or not lse.is_contiguous()):
-        raise ValueError(f"lse must be a contiguous float32 ({hq}, {tokens}) tensor")
-    return tokens, hq, dim, o
+    if rc != _lib.OK:
+        _lib.check(rc, call.__name__)
+    if out is not o:
+        o.copy_(out)
+    return o
 
 
 def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -229,34 +239,30 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
     are reported by ``ops.check_status``.
     """
     dev = _require_cuda(q, k, v, cu_seqlens, o, lse)
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape:
+    kv_shape = k.shape
+    if len(kv_shape) != 3 or kv_shape != v.shape:
         raise ValueError("q, k and v must be (tokens, heads, head_dim), k and v of one shape")
-    tokens, hq, dim, o = _check_packed(q, k.shape[1], o, lse)
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    tokens, hq, dim, dtype = _check_packed(q, kv_shape[1], o, lse)
+    if k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise ValueError("q, k and v must share one dtype, float16 or bfloat16")
-    if k.shape[0] != tokens or k.shape[2] != dim:
-        raise ValueError(f"k/v shape {tuple(k.shape)} does not match q {tuple(q.shape)}")
+    if kv_shape[0] != tokens or kv_shape[2] != dim:
+        raise ValueError(f"k/v shape {tuple(kv_shape)} does not match q {tuple(q.shape)}")
     cu_seqlens = _int_vector(cu_seqlens, None, torch.int32, "cu_seqlens")
     prompts = cu_seqlens.shape[0] - 1
     if prompts < 0:
         raise ValueError("cu_seqlens needs at least one entry")
     if tokens == 0 or prompts == 0:
-        return o
-    q, k, v = _readable(q), _readable(k), _readable(v)
-    out = o if _packed(o) else torch.empty(o.shape, dtype=o.dtype, device=dev)
-    if out is not o:
-        out.copy_(o)  # rows past the last prompt keep what o holds
-    strides = _I64x8(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *out.stride()[:2])
+        return torch.empty_like(q) if o is None else o
+    (q, q_token, q_head), (k, k_token, k_head), (v, v_token, v_head) = _packed(q), _packed(k), _packed(v)
     handle = _lib.lib()
-    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), strides,
-            cu_seqlens.data_ptr(), prompts, tokens, hq, k.shape[1], dim, _DT[q.dtype],
-            dim ** -0.5 if sm_scale is None else sm_scale, None if lse is None else lse.data_ptr())
-    rc = _with_workspace(handle.b2g_attention_prefill, args, dev,
-                         lambda: handle.b2g_attention_prefill_workspace_bytes(prompts, tokens, hq))
-    _lib.check(rc, "b2g_attention_prefill")
-    if out is not o:
-        o.copy_(out)
-    return o
+    return _run_packed(
+        handle.b2g_attention_prefill,
+        lambda: handle.b2g_attention_prefill_workspace_bytes(prompts, tokens, hq), dev, q, o, lse,
+        lambda out, o_token, o_head, lse_ptr: (
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out,
+            _I64x8(q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head),
+            cu_seqlens.data_ptr(), prompts, tokens, hq, kv_shape[1], dim, dtype,
+            dim ** -0.5 if sm_scale is None else sm_scale, lse_ptr))
 
 
 def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -282,14 +288,12 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     current stream; bad pages and lengths are reported by ``ops.check_status``.
     """
     dev = _require_cuda(q, k_cache, v_cache, block_tables, seq_lens, cu_seqlens, tree_mask, o, lse)
-    if q.dim() != 3:
-        raise ValueError("q must be (tokens, heads, head_dim)")
     check_caches(k_cache, v_cache, q.dtype)
     pages, page, hk, cache_dim = k_cache.shape
-    tokens, hq, dim, o = _check_packed(q, hk, o, lse)
+    tokens, hq, dim, dtype = _check_packed(q, hk, o, lse)
     if cache_dim != dim:
         raise ValueError(f"q has heads of {dim}, the cache of {cache_dim}")
-    if block_tables.dim() != 2 or block_tables.dtype != torch.int32:
+    if block_tables.dtype is not torch.int32 or len(block_tables.shape) != 2:
         raise ValueError("block_tables must be a 2-D int32 tensor")
     requests, max_pages = block_tables.shape
     table_stride, column_stride = block_tables.stride()
@@ -298,35 +302,29 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         table_stride = max_pages
     seq_lens = _int_vector(seq_lens, requests, torch.int32, "seq_lens")
     cu_seqlens = _int_vector(cu_seqlens, requests + 1, torch.int32, "cu_seqlens")
-    words = 0
+    mask_ptr, words = None, 0
     if tree_mask is not None:
-        if tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != tokens:
+        if tree_mask.dtype is not torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != tokens:
             raise ValueError(f"tree_mask must be an int64 ({tokens}, words) tensor")
         words = tree_mask.shape[1]
         if words < 1:
             raise ValueError("tree_mask needs at least one word per token")
         tree_mask = tree_mask.contiguous()
+        mask_ptr = tree_mask.data_ptr()
     if tokens == 0 or requests == 0:
-        return o
-    q = _readable(q)
-    out = o if _packed(o) else torch.empty(o.shape, dtype=o.dtype, device=dev)
-    if out is not o:
-        out.copy_(o)  # rows past the last request keep what o holds
-    strides = _I64x10(*q.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3],
-                      *out.stride()[:2])
+        return torch.empty_like(q) if o is None else o
+    q, q_token, q_head = _packed(q)
     handle = _lib.lib()
-    args = (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), strides,
+    return _run_packed(
+        handle.b2g_attention_tree,
+        lambda: handle.b2g_attention_tree_workspace_bytes(requests, tokens, hq, hk, dim), dev, q, o,
+        lse,
+        lambda out, o_token, o_head, lse_ptr: (
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out,
+            _I64x10(q_token, q_head, *k_cache.stride()[:3], *v_cache.stride()[:3], o_token, o_head),
             block_tables.data_ptr(), table_stride, max_pages, seq_lens.data_ptr(),
-            cu_seqlens.data_ptr(), None if tree_mask is None else tree_mask.data_ptr(), words,
-            requests, tokens, hq, hk, dim, pages, page, _DT[q.dtype],
-            dim ** -0.5 if sm_scale is None else sm_scale, None if lse is None else lse.data_ptr())
-    rc = _with_workspace(handle.b2g_attention_tree, args, dev,
-                         lambda: handle.b2g_attention_tree_workspace_bytes(requests, tokens, hq,
-                                                                           hk, dim))
-    _lib.check(rc, "b2g_attention_tree")
-    if out is not o:
-        o.copy_(out)
-    return o
+            cu_seqlens.data_ptr(), mask_ptr, words, requests, tokens, hq, hk, dim, pages, page,
+            dtype, dim ** -0.5 if sm_scale is None else sm_scale, lse_ptr))
 
 
 def main(argv=None) -> None:

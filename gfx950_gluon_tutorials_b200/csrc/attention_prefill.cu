@@ -15,9 +15,10 @@
 //     key/value head, where neighbouring heads would need two tiles of K and V.
 //   - with an odd number, blocks of up to 128 rows are kHeads items too, whose heads
 //     may then differ in K and V: every KV tile takes two ring stages.
-// A planning kernel (packed_plan_kernel) lists the blocks in order of falling work;
-// they are dealt to the CTAs in turns of alternating direction, which evens out
-// their sums.
+// The blocks are listed in order of falling work and dealt to the CTAs in turns of
+// alternating direction, which evens out their sums. Up to kOwnBlocks of them every
+// CTA makes the list for itself (one prompt of 61 tokens: PLAN_OWN us on the GPU against
+// PLAN_KERNEL with a planning launch), above that a planning kernel does.
 //
 // What bounds it: the two products and the exponentials of a tile, as in
 // attention.cu, and for short prompts the hand-over from item to item.
@@ -44,12 +45,16 @@ struct alignas(64) PrefillParams {
   int64_t v_t, v_h;
   float* lse;                 // [HQ][tokens] or null
   int* status;
-  const int4* plan;           // blocks: {first token, its row in the prompt, prompt's rows, 0}
+  const int32_t* cu;
+  const int4* plan;           // blocks: {first token, its row in the prompt, prompt's rows, 0}; null: own list
   const int2* counts;         // kRows blocks (first in the plan), kHeads blocks
-  int32_t HQ, G, tokens;
+  int32_t HQ, G, tokens, prompts, block;
   float scale_log2;
   uint64_t timeout_ns;
 };
+
+constexpr uint32_t kOwnBlocks = 256;   // most blocks that a CTA lists for itself
+constexpr int32_t kPlanLevels = 4096;  // levels of work: KV tiles of 128 keys, half a million tokens
 
 template <int D>
 struct PrefillPlan {
@@ -67,7 +72,9 @@ struct PrefillPlan {
   static constexpr uint32_t kNumBars = 2 + 4 * kStages + 10;
   static constexpr uint32_t kMiscOff = kBarOff + kNumBars * 8;  // tmem slot, abort flag
   static constexpr uint32_t kOddOff = kMiscOff + 16;            // [3][2 items][4 warps], see odd_words
-  static constexpr uint32_t kBytes = kOddOff + 96;
+  // a CTA's own list: int4 sorted[kOwnBlocks], unsorted[kOwnBlocks], int32 keys[kOwnBlocks]
+  static constexpr uint32_t kListOff = (kOddOff + 96 + 15) / 16 * 16;
+  static constexpr uint32_t kBytes = kListOff + kOwnBlocks * 36;
   static constexpr uint32_t kDynBytes = kBytes + 1024;  // + alignment slack
   static constexpr uint32_t kS = 0, kO = 256, kTileCols = 128;  // TMEM columns, as in attention.cu
   static_assert(kDynBytes <= 232448, "shared memory");
@@ -95,7 +102,25 @@ __device__ __noinline__ void add_odd_values(const PrefillParams& p, int32_t t0, 
 // CTA; latency-bound (three passes over the offsets). The order only decides which
 // CTA works when, never a result.
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanLevels = 4096;  // KV tiles of 128 keys: half a million tokens
+
+// Rows of prompt b and its first token. Offsets are 0 <= cu[0] <= cu[1] <= ... <= tokens;
+// others are cut to that and reported.
+__device__ __forceinline__ int32_t prompt_rows(const int32_t* cu, int b, int32_t tokens,
+                                               int* status, int32_t& begin) {
+  const int32_t lo = cu[b], hi = cu[b + 1];
+  begin = min(max(lo, 0), tokens);
+  if ((lo < 0 || hi < lo || hi > tokens) && status != nullptr)
+    atomicCAS(status, 0, B2G_STATUS_TOKENS);
+  return min(max(hi, begin), tokens) - begin;
+}
+
+// Where the block at `row` of a prompt belongs: kRows blocks first, falling work is
+// rising level.
+__device__ __forceinline__ int32_t block_level(int32_t row, int32_t rows, int32_t block) {
+  const bool two = block == 256 && rows - row > 128;
+  const int32_t kv = row / 128 + (two ? 2 : 1);
+  return kPlanLevels - min(kv, kPlanLevels) + (two ? 0 : kPlanLevels);
+}
 
 struct PackedPlanParams {
   const int32_t* cu;
@@ -114,25 +139,12 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PackedP
   grid_launch_dependents();
   for (int i = threadIdx.x; i < 2 * kPlanLevels; i += kPlanThreads) level[i] = 0;
   __syncthreads();
-  // offsets are 0 <= cu[0] <= cu[1] <= ... <= tokens; others are cut to that
-  auto prompt = [&](int b, int32_t& begin, int32_t& rows) {
-    const int32_t lo = p.cu[b], hi = p.cu[b + 1];
-    begin = min(max(lo, 0), p.tokens);
-    rows = min(max(hi, begin), p.tokens) - begin;
-    if ((lo < 0 || hi < lo || hi > p.tokens) && p.status != nullptr)
-      atomicCAS(p.status, 0, B2G_STATUS_TOKENS);
-  };
-  // a warp to a prompt, a lane to a block; falling work is rising level here
-  auto level_of = [](int32_t row, int32_t rows, int32_t block) {
-    const bool two = block == 256 && rows - row > 128;
-    const int32_t kv = row / 128 + (two ? 2 : 1);
-    return kPlanLevels - min(kv, kPlanLevels) + (two ? 0 : kPlanLevels);
-  };
+  // a warp to a prompt, a lane to a block
   for (int b = warp; b < p.prompts; b += kPlanThreads / 32) {
-    int32_t begin, rows;
-    prompt(b, begin, rows);
+    int32_t begin;
+    const int32_t rows = prompt_rows(p.cu, b, p.tokens, p.status, begin);
     for (int32_t row = lane * p.block; row < rows; row += 32 * p.block)
-      atomicAdd(&level[level_of(row, rows, p.block)], 1);
+      atomicAdd(&level[block_level(row, rows, p.block)], 1);
   }
   __syncthreads();
   // exclusive sums over the levels, eight to a thread
@@ -165,13 +177,63 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PackedP
   }
   __syncthreads();
   for (int b = warp; b < p.prompts; b += kPlanThreads / 32) {
-    int32_t begin, rows;
-    prompt(b, begin, rows);
+    int32_t begin;
+    const int32_t rows = prompt_rows(p.cu, b, p.tokens, p.status, begin);
     for (int32_t row = lane * p.block; row < rows; row += 32 * p.block) {
-      const int32_t at = atomicAdd(&level[level_of(row, rows, p.block)], 1);
+      const int32_t at = atomicAdd(&level[block_level(row, rows, p.block)], 1);
       if (at < p.capacity) p.plan[at] = make_int4(begin + row, row, rows, 0);
     }
   }
+}
+
+// The same list, made by one CTA of the attention kernel for itself: up to kOwnBlocks
+// blocks of at most as many prompts as it has threads. All CTAs have to come to the
+// same order, so blocks of equal level keep the order of the prompts: a block's place
+// is the number of blocks before it. Returns the counts; all threads take part.
+template <int kThreads>
+__device__ __forceinline__ int2 list_own_blocks(const PrefillParams& p, int4* sorted, int4* raw,
+                                                int32_t* keys) {
+  static_assert(kOwnBlocks <= kThreads, "one block to a thread");
+  __shared__ int32_t warp_sum[kThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b = static_cast<int>(threadIdx.x);
+  int32_t begin = 0, rows = 0;
+  if (b < p.prompts)
+    rows = prompt_rows(p.cu, b, p.tokens, blockIdx.x == 0 ? p.status : nullptr, begin);
+  const int32_t n = (rows + p.block - 1) / p.block;
+  int32_t at = n;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int32_t up = __shfl_up_sync(0xffffffffu, at, d);
+    if (lane >= d) at += up;
+  }
+  if (lane == 31) warp_sum[warp] = at;
+  __syncthreads();
+  int32_t total = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) at += warp_sum[w];
+    total += warp_sum[w];
+  }
+  total = min(total, static_cast<int32_t>(kOwnBlocks));  // decreasing offsets can ask for more
+  at -= n;
+  for (int32_t i = 0; i < n && at + i < total; ++i) {
+    raw[at + i] = make_int4(begin + i * p.block, i * p.block, rows, 0);
+    keys[at + i] = block_level(i * p.block, rows, p.block);
+  }
+  __syncthreads();
+  const bool mine = b < total;
+  const int32_t key = mine ? keys[b] : 0;
+  if (mine) {
+    int32_t place = 0;
+#pragma unroll 4
+    for (int32_t f = 0; f < total; ++f) {
+      const int32_t other = keys[f];
+      place += other < key || (other == key && f < b) ? 1 : 0;
+    }
+    sorted[place] = raw[b];
+  }
+  const int32_t twos = __syncthreads_count(mine && key < kPlanLevels);
+  return make_int2(twos, total - twos);
 }
 
 // ----------------------------------------------------------------- kernel --
@@ -203,47 +265,40 @@ struct PrefillItem {
   }
 };
 
-// Walks a CTA's items; the plan's entry of the next one is loaded an item ahead.
+// Walks a CTA's items. What it needs of the list stays in shared memory or is
+// prefetched an item ahead: registers are the softmax's.
 struct PrefillWalk {
-  int32_t item, items, row_blocks, row_items, pairs;
+  int32_t item;
   uint32_t turn;
-  int4 ahead;
 
-  __device__ __forceinline__ void begin(const PrefillParams& p) {
-    const int2 c = *p.counts;
-    pairs = (p.HQ + 1) / 2;
-    row_blocks = c.x;
-    row_items = c.x * p.HQ;
-    items = row_items + c.y * pairs;
-    item = static_cast<int32_t>(blockIdx.x);
-    turn = 0;
-    fetch(p);
-  }
-  __device__ __forceinline__ void fetch(const PrefillParams& p) {
-    if (item < items)
-      ahead = p.plan[item < row_items ? item / p.HQ : row_blocks + (item - row_items) / pairs];
-  }
-  __device__ __forceinline__ bool next(const PrefillParams& p, PrefillItem& w) {
+  __device__ __forceinline__ bool next(const PrefillParams& p, const int4* own, const int2* counts,
+                                       PrefillItem& w) {
+    const int4* list = p.plan == nullptr ? own : p.plan;
+    const int32_t pairs = (p.HQ + 1) / 2, row_blocks = counts->x, row_items = row_blocks * p.HQ;
+    const int32_t items = row_items + counts->y * pairs;
+    auto entry = [&](int32_t i) { return i < row_items ? i / p.HQ : row_blocks + (i - row_items) / pairs; };
     if (item >= items) return false;
+    const int4 e = list[entry(item)];
     w.by_rows = item < row_items;
-    w.m0 = ahead.x;
-    w.k0 = ahead.x - ahead.y;
-    w.rows = ahead.z - ahead.y;
+    w.m0 = e.x;
+    w.k0 = e.x - e.y;
+    w.rows = e.z - e.y;
     if (w.by_rows) {
       w.head = item % p.HQ;
       w.slots = 2;
       w.shared = true;
-      w.n = ahead.y / 128 + 2;
+      w.n = e.y / 128 + 2;
     } else {
       w.head = 2 * ((item - row_items) % pairs);
       w.slots = w.head + 1 < p.HQ ? 2u : 1u;
       w.shared = w.slots == 1u || w.head / p.G == (w.head + 1) / p.G;
-      w.n = ahead.y / 128 + 1;
+      w.n = e.y / 128 + 1;
     }
     const int32_t g = static_cast<int32_t>(gridDim.x), c = static_cast<int32_t>(blockIdx.x);
     item += (turn & 1u) ? 2 * c + 1 : 2 * (g - c) - 1;
     ++turn;
-    fetch(p);
+    if (p.plan != nullptr && item < items)
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(p.plan + entry(item)));
     return true;
   }
 };
@@ -300,13 +355,21 @@ __global__ void __launch_bounds__(PrefillPlan<D>::kThreads, 1)
     tmem_alloc<1>(smem_u32(tmem_slot), 512);
     tmem_relinquish<1>();
   }
+  int4* own_list = reinterpret_cast<int4*>(smem + PP::kListOff);
+  int2* counts = reinterpret_cast<int2*>(smem + PP::kMiscOff + 8);
+  if (p.plan == nullptr) {
+    const int2 c = list_own_blocks<PP::kThreads>(
+        p, own_list, own_list + kOwnBlocks, reinterpret_cast<int32_t*>(own_list + 2 * kOwnBlocks));
+    if (threadIdx.x == 0) *counts = c;
+  } else {
+    grid_dependency_wait();  // the plan is complete
+    if (threadIdx.x == 0) *counts = *p.counts;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-  grid_dependency_wait();  // the plan is complete
-  PrefillWalk walk;
-  walk.begin(p);
+  PrefillWalk walk = {static_cast<int32_t>(blockIdx.x), 0u};
   PrefillItem w;
 
   if (warp == 0) {
@@ -315,7 +378,7 @@ __global__ void __launch_bounds__(PrefillPlan<D>::kThreads, 1)
       uint32_t base = 0, ic = 0;  // ring stages before the item, items
       uint32_t nk = 0, nv = 0;    // K and V loads issued
       bool alive = true;
-      while (alive && walk.next(p, w)) {
+      while (alive && walk.next(p, own_list, counts, w)) {
         if (ic > 0 && !fmha_wait(q_empty, (ic - 1u) & 1u, abort_flag, p, B2G_SITE_EMPTY)) break;
         mbar_arrive_expect_tx(q_full, w.slots * PP::kTile);
         for (uint32_t t = 0; t < w.slots; ++t)
@@ -400,7 +463,9 @@ __global__ void __launch_bounds__(PrefillPlan<D>::kThreads, 1)
         }
         commit(s_full(t));
       };
-      while (alive && walk.next(p, w)) {
+      // (uniform: where the compiler cannot see that the warp stays converged, issuing is
+      // as slow as from one thread)
+      while (alive && uniform(static_cast<int32_t>(walk.next(p, own_list, counts, w))) != 0) {
         w.n = uniform(w.n);
         w.slots = uniform(w.slots);
         w.shared = uniform(static_cast<int32_t>(w.shared)) != 0;
@@ -491,7 +556,7 @@ __global__ void __launch_bounds__(PrefillPlan<D>::kThreads, 1)
     auto wait_all = [&](uint32_t bar, uint32_t parity, int site) {
       return __all_sync(0xffffffffu, fmha_wait(bar, parity & 1u, abort_flag, p, site)) != 0;
     };
-    while (alive && walk.next(p, w)) {
+    while (alive && walk.next(p, own_list, counts, w)) {
       const uint32_t stage0 = base;
       base += w.stages();
       if (t >= w.slots) continue;
@@ -606,7 +671,7 @@ int launch_prefill(const PrefillParams& prm, int64_t items, int sms, cudaStream_
       return static_cast<int>(cudaGetLastError());
     attr_set[dev].store(true);
   }
-  // set up while the planning kernel runs; grid_dependency_wait orders the rest
+  // after a planning kernel: set up while it runs, grid_dependency_wait orders the rest
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(items, sms)), 1, 1);
   cfg.blockDim = dim3(PP::kThreads, 1, 1);
@@ -616,7 +681,7 @@ int launch_prefill(const PrefillParams& prm, int64_t items, int sms, cudaStream_
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = prm.plan != nullptr ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, prm);
   if (e != cudaSuccess) cudaGetLastError();
   return e == cudaSuccess ? B2G_OK : static_cast<int>(e);
@@ -676,18 +741,27 @@ extern "C" int b2g_attention_prefill(const void* q, const void* k, const void* v
   if (!encode(&prm.tmQ, q, heads_q, strides) || !encode(&prm.tmK, k, heads_k, strides + 2) ||
       !encode(&prm.tmV, v, heads_k, strides + 4))
     return B2G_ETENSORMAP;
-  uint8_t* ws = static_cast<uint8_t*>(workspace) + workspace_flag_bytes(sms);
-  PackedPlanParams pl;
-  pl.cu = cu_seqlens;
-  pl.counts = reinterpret_cast<int2*>(ws);
-  pl.plan = reinterpret_cast<int4*>(ws + 256);
-  pl.status = status;
-  pl.prompts = prompts;
-  pl.tokens = static_cast<int32_t>(tokens);
-  pl.capacity = static_cast<int32_t>(blocks);
-  pl.block = block_rows(group);
-  prm.plan = pl.plan;
-  prm.counts = pl.counts;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  prm.cu = cu_seqlens;
+  prm.prompts = prompts;
+  prm.block = block_rows(group);
+  if (blocks > static_cast<int64_t>(kOwnBlocks) || prompts > PrefillPlan<128>::kThreads) {
+    uint8_t* ws = static_cast<uint8_t*>(workspace) + workspace_flag_bytes(sms);
+    PackedPlanParams pl;
+    pl.cu = cu_seqlens;
+    pl.counts = reinterpret_cast<int2*>(ws);
+    pl.plan = reinterpret_cast<int4*>(ws + 256);
+    pl.status = status;
+    pl.prompts = prompts;
+    pl.tokens = static_cast<int32_t>(tokens);
+    pl.capacity = static_cast<int32_t>(blocks);
+    pl.block = prm.block;
+    prm.plan = pl.plan;
+    prm.counts = pl.counts;
+    packed_plan_kernel<<<1, kPlanThreads, 0, s>>>(pl);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
   prm.O = o;
   prm.o_t = strides[6];
   prm.o_h = strides[7];
@@ -701,10 +775,6 @@ extern "C" int b2g_attention_prefill(const void* q, const void* k, const void* v
   prm.tokens = static_cast<int32_t>(tokens);
   prm.scale_log2 = sm_scale * 1.4426950408889634f;
   prm.timeout_ns = wait_timeout_ns();
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  packed_plan_kernel<<<1, kPlanThreads, 0, s>>>(pl);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return static_cast<int>(e);
   const bool bf16 = dtype == B2G_DT_BF16;
   const int64_t items = blocks * heads_q;  // at most
   if (head_dim == 128)

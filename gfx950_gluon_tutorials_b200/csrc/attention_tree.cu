@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
       const uint64_t q_desc = sdesc_kmajor_sw128(sbase + TP::kQOff);
       const uint64_t k_desc = sdesc_kmajor_sw128(sbase + TP::kRingOff);
       const uint64_t v_desc = sdesc_mnmajor_sw128(sbase + TP::kRingOff, kSlabBytes, 1024u);
-      while (alive && walk.next(p, w)) {
+      while (alive && uniform(static_cast<int32_t>(walk.next(p, w))) != 0) {
         const int32_t n = uniform(w.j1 - w.j0);
         const bool two = uniform(static_cast<int32_t>(w.two)) != 0;
         const uint32_t slots = two || n > 1 ? 2u : 1u;

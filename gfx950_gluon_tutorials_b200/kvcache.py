@@ -28,6 +28,7 @@ from .ops import _require_cuda, _stream_handle, status_tensor
 _DT = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
 MAX_REQUESTS = 8192
 _I64x10 = ctypes.c_int64 * 10
+_ONE = torch.Size([1])
 
 
 class StepMaps(NamedTuple):
@@ -66,23 +67,30 @@ def map_step(cached_lens: torch.Tensor, new_lens: torch.Tensor, page_counts: tor
     returned ``num_free`` is minus the number of missing pages. All lengths,
     counts and tables are int32 CUDA tensors, ``num_free`` of shape (1,)."""
     dev = _require_cuda(cached_lens, new_lens, page_counts, block_tables, free_pages, num_free)
-    if block_tables.dim() != 2 or block_tables.dtype != torch.int32:
+    i32 = torch.int32
+    if block_tables.dtype is not i32 or len(block_tables.shape) != 2:
         raise ValueError("block_tables must be a 2-D int32 tensor")
+    per_request = block_tables.shape[:1]
     requests, max_pages = block_tables.shape
     table_stride, column_stride = block_tables.stride()
     if max_pages > 1 and column_stride != 1:
         raise ValueError("block_tables is updated in place: its rows must be contiguous")
-    cached_lens = _int_vector(cached_lens, requests, torch.int32, "cached_lens")
-    new_lens = _int_vector(new_lens, requests, torch.int32, "new_lens")
-    page_counts = _int_vector(page_counts, requests, torch.int32, "page_counts")
-    free_pages = _int_vector(free_pages, None, torch.int32, "free_pages")
-    num_free = _int_vector(num_free, 1, torch.int32, "num_free")
+    if not (cached_lens.dtype is new_lens.dtype is page_counts.dtype is free_pages.dtype is num_free.dtype is i32
+            and cached_lens.shape == new_lens.shape == page_counts.shape == per_request
+            and len(free_pages.shape) == 1 and num_free.shape == _ONE
+            and cached_lens.is_contiguous() and new_lens.is_contiguous()
+            and page_counts.is_contiguous() and free_pages.is_contiguous()):
+        cached_lens = _int_vector(cached_lens, requests, i32, "cached_lens")
+        new_lens = _int_vector(new_lens, requests, i32, "new_lens")
+        page_counts = _int_vector(page_counts, requests, i32, "page_counts")
+        free_pages = _int_vector(free_pages, None, i32, "free_pages")
+        num_free = _int_vector(num_free, 1, i32, "num_free")
     if page_size < 1 or num_tokens < 0:
         raise ValueError("page_size must be positive and num_tokens not negative")
     # one allocation for the int32 outputs
     n = num_tokens
     slots = torch.empty(n, dtype=torch.int64, device=dev)
-    ints = torch.empty(n + 3 * requests + 2, dtype=torch.int32, device=dev)
+    ints = torch.empty(n + 3 * requests + 2, dtype=i32, device=dev)
     positions, cu, seq, counts, left = ints.split_with_sizes(
         (n, requests + 1, requests, requests, 1))
     base = ints.data_ptr()
@@ -99,11 +107,12 @@ def map_step(cached_lens: torch.Tensor, new_lens: torch.Tensor, page_counts: tor
 
 def check_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype: torch.dtype) -> None:
     """Both caches 4-D, of one shape and ``dtype``, with unit stride along the head dim."""
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+    shape = k_cache.shape
+    if len(shape) != 4 or shape != v_cache.shape:
         raise ValueError("k_cache and v_cache must share one shape (pages, page_size, heads, head_dim)")
-    if k_cache.dtype != dtype or v_cache.dtype != dtype:
+    if k_cache.dtype is not dtype or v_cache.dtype is not dtype:
         raise ValueError(f"the caches must hold {dtype}, got {k_cache.dtype} and {v_cache.dtype}")
-    if k_cache.shape[3] > 1 and (k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
+    if shape[3] > 1 and (k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
         raise ValueError("the caches must be contiguous along the head dim")
 
 
@@ -114,9 +123,10 @@ def write_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     skipped and reported by ``ops.check_status``. ``k`` and ``v`` may be views of a
     fused projection's output (unit stride along the head dim)."""
     dev = _require_cuda(k, v, k_cache, v_cache, slots)
-    if k.dtype not in _DT or v.dtype != k.dtype:
+    dtype = _DT.get(k.dtype)
+    if dtype is None or v.dtype is not k.dtype:
         raise ValueError("k and v must share one dtype, float16 or bfloat16")
-    if k.dim() != 3 or k.shape != v.shape:
+    if len(k.shape) != 3 or k.shape != v.shape:
         raise ValueError("k and v must share one shape (tokens, heads, head_dim)")
     check_caches(k_cache, v_cache, k.dtype)
     tokens, heads, dim = k.shape
@@ -126,14 +136,15 @@ def write_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     slots = _int_vector(slots, tokens, torch.int64, "slots")
     if tokens == 0:
         return
-    if k.stride(2) != 1:
-        k = k.contiguous()
-    if v.stride(2) != 1:
-        v = v.contiguous()
-    strides = _I64x10(*k.stride()[:2], *v.stride()[:2], *k_cache.stride()[:3],
+    (k_token, k_head, k_dim), (v_token, v_head, v_dim) = k.stride(), v.stride()
+    if k_dim != 1 or v_dim != 1:
+        k, v = k.contiguous(), v.contiguous()
+        k_token = v_token = heads * dim
+        k_head = v_head = dim
+    strides = _I64x10(k_token, k_head, v_token, v_head, *k_cache.stride()[:3],
                       *v_cache.stride()[:3])
     rc = _lib.lib().b2g_kv_write(
         k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), strides,
-        slots.data_ptr(), tokens, heads, dim, pages, page, _DT[k.dtype],
+        slots.data_ptr(), tokens, heads, dim, pages, page, dtype,
         status_tensor(dev).data_ptr(), _stream_handle(dev))
     _lib.check(rc, "b2g_kv_write")

@@ -37,6 +37,13 @@ def _stream_handle(device: torch.device) -> int:
 
 def _require_cuda(*ts: torch.Tensor) -> torch.device:
     dev = ts[0].device
+    index = ts[0].get_device()  # -1 on the host
+    if index >= 0:
+        for t in ts:
+            if t is not None and t.get_device() != index:
+                break
+        else:
+            return dev
     for t in ts:
         if t is None:
             continue
