@@ -12,7 +12,8 @@
 // (block, head, tile), are one list that is cut into equal shares, one per CTA
 // (one per SM); every CTA adds up the requests' tiles itself to find where its
 // share begins, which costs about a microsecond where a planning launch of its
-// own cost five. So a batch of uneven lengths and a single long request alike keep
+// own cost five. Beginning a block costs a CTA about as much as kBlockCost tiles,
+// which the list holds ahead of each block's. So a batch of uneven lengths and a single long request alike keep
 // every SM reading to the end. A block whose tiles lie in several shares is
 // joined at the end: each CTA publishes its rows of O with their maxima and sums,
 // and when all have, each joins its slice of the rows, in a fixed order.
@@ -55,11 +56,11 @@ struct TreeEntry {
   int32_t len;              // keys
 };
 
-// Where a share begins: head and tile of `e`; `before` units lie before the block.
+// Where a share begins: head of `e` and unit of that; `before` units lie before the block.
 struct ShareStart {
   int64_t units, before, here;  // here: units of the share
   TreeEntry e;
-  int32_t hk, tile;
+  int32_t hk, unit;
 };
 
 struct alignas(64) TreeParams {
@@ -77,8 +78,10 @@ struct alignas(64) TreeParams {
   int* status;
   const int32_t* cu;
   const int32_t* lens;
-  float* part;             // [2 per CTA][D / 4][part_rows] float4: unfinished O, rows side by side
-  float2* part_ml;         // [2 per CTA][part_rows] {max (log2 units), sum}
+  // Parts of unfinished blocks, four per CTA: of the block that its share begins
+  // inside and of the one that it ends inside, of each warpgroup
+  float* part;             // [4 per CTA][D / 4][part_rows] float4: O, rows side by side
+  float2* part_ml;         // [4 per CTA][part_rows] {max (log2 units), sum}
   uint32_t* counters;      // two per CTA, zero at rest: published, joined
   int32_t mask_words, part_rows, requests;
   int32_t most;            // keys that a table has room for
@@ -87,10 +90,13 @@ struct alignas(64) TreeParams {
   uint64_t timeout_ns;
 };
 
+constexpr int32_t kBlockCost = 8;
+
 template <int D>
 struct TreePlan {
   static constexpr uint32_t kSoftmaxWarps = 8;
-  static constexpr uint32_t kThreads = 64 + 32 * kSoftmaxWarps;
+  static constexpr uint32_t kFirstSoftmax = 2;  // after the producer and the MMA issuer
+  static constexpr uint32_t kThreads = 32 * (kFirstSoftmax + kSoftmaxWarps);
   static constexpr uint32_t kSlabs = D / 64;
   static constexpr uint32_t kTile = kSlabs * kSlabBytes;  // Q, K or V tile
   static constexpr uint32_t kSlots = D == 128 ? 5 : 10;   // ring of K and V tiles in turn
@@ -174,7 +180,7 @@ __device__ __forceinline__ void find_share(const TreeParams& p, int64_t* sums, S
     const TreeEntry e = tree_request(p, r, report);
     const int32_t blocks = tree_blocks(p, e);
     int64_t n = 0;
-    for (int32_t b = 0; b < blocks; ++b) n += tree_tiles(p, e, b);
+    for (int32_t b = 0; b < blocks; ++b) n += tree_tiles(p, e, b) + kBlockCost;
     return n;
   };
   int64_t first = 0, sum = 0;  // this thread's first request, and all of them
@@ -210,23 +216,23 @@ __device__ __forceinline__ void find_share(const TreeParams& p, int64_t* sums, S
     out->here = 0;
   }
   if (static_cast<int64_t>(blockIdx.x) >= ctas) return;
-  int64_t n = first, before = base + scan - first;  // tiles of this thread's request, and before it
+  int64_t n = first, before = base + scan - first;  // units a head of this thread's request, and before it
   for (int32_t r0 = 0;;) {
     if (n > 0 && before * p.HK <= u && u < (before + n) * p.HK) {
       const int32_t r = r0 + static_cast<int32_t>(threadIdx.x);
       TreeEntry e = tree_request(p, r, false);
       e.tiles = tree_tiles(p, e, 0);
-      while (u >= (before + e.tiles) * p.HK) {
-        before += e.tiles;
+      while (u >= (before + e.tiles + kBlockCost) * p.HK) {
+        before += e.tiles + kBlockCost;
         e.tiles = tree_tiles(p, e, ++e.block);
       }
-      const int64_t in = u - before * p.HK;  // less than tiles * HK
+      const int64_t in = u - before * p.HK;  // less than (tiles + kBlockCost) * HK
       out->here = share_begin(units, static_cast<int32_t>(blockIdx.x) + 1,
                               static_cast<int32_t>(ctas)) - u;
       out->before = before * p.HK;
       out->e = e;
-      out->hk = static_cast<int32_t>(mul_div(in, 1, e.tiles));
-      out->tile = static_cast<int32_t>(in - static_cast<int64_t>(out->hk) * e.tiles);
+      out->hk = static_cast<int32_t>(mul_div(in, 1, e.tiles + kBlockCost));
+      out->unit = static_cast<int32_t>(in - static_cast<int64_t>(out->hk) * (e.tiles + kBlockCost));
     }
     r0 += static_cast<int32_t>(kThreads);
     // the same for all threads: whether the share begins in a later round of requests
@@ -254,7 +260,7 @@ __device__ __forceinline__ void find_share(const TreeParams& p, int64_t* sums, S
 // The part of one (block, key/value head) that lies in this CTA's share.
 struct Segment {
   TreeEntry e;
-  int64_t unit0;    // the block and head's first unit
+  int64_t unit0;    // the unit of the block and head's first tile
   int32_t hk;
   int32_t j0, j1;   // tiles
   int32_t row0, rows;
@@ -266,42 +272,46 @@ struct Segment {
 struct SegmentWalk {
   TreeEntry e;
   int64_t left, before;  // before: units before the block
-  int32_t hk, tile;
+  int32_t hk, unit;
 
   __device__ __forceinline__ void begin(const ShareStart& s) {
     left = s.here;
     before = s.before;
     e = s.e;
     hk = s.hk;
-    tile = s.tile;
+    unit = s.unit;
   }
 
   __device__ __forceinline__ bool next(const TreeParams& p, Segment& s) {
-    if (left <= 0) return false;
-    if (hk == p.HK) {  // the next block, of this request or of the next that has new tokens
-      before += static_cast<int64_t>(e.tiles) * p.HK;
-      hk = 0;
-      if (e.block + 1 < tree_blocks(p, e)) {
-        ++e.block;
-      } else {
-        do e = tree_request(p, e.request + 1, false);
-        while (e.fresh == 0);
+    while (left > 0) {
+      if (hk == p.HK) {  // the next block, of this request or of the next that has new tokens
+        before += static_cast<int64_t>(e.tiles + kBlockCost) * p.HK;
+        hk = 0;
+        if (e.block + 1 < tree_blocks(p, e)) {
+          ++e.block;
+        } else {
+          do e = tree_request(p, e.request + 1, false);
+          while (e.fresh == 0);
+        }
+        e.tiles = tree_tiles(p, e, e.block);
       }
-      e.tiles = tree_tiles(p, e, e.block);
+      const int32_t of_head = e.tiles + kBlockCost, from = unit;
+      const int32_t to = static_cast<int32_t>(min(static_cast<int64_t>(of_head), from + left));
+      left -= to - from;
+      unit = 0;
+      s.hk = hk++;
+      if (to <= kBlockCost) continue;  // the share ends before the block's first tile
+      s.e = e;
+      s.unit0 = before + static_cast<int64_t>(s.hk) * of_head + kBlockCost;
+      s.j0 = max(from - kBlockCost, 0);
+      s.j1 = to - kBlockCost;
+      s.row0 = e.block * 256;
+      s.rows = min(256, e.fresh * p.G - s.row0);
+      s.two = s.rows > 128;
+      s.slots = s.two || s.j1 - s.j0 > 1 ? 2u : 1u;
+      return true;
     }
-    s.e = e;
-    s.hk = hk;
-    s.unit0 = before + static_cast<int64_t>(hk) * e.tiles;
-    s.j0 = tile;
-    s.j1 = static_cast<int32_t>(min(static_cast<int64_t>(e.tiles), tile + left));
-    left -= s.j1 - s.j0;
-    s.row0 = e.block * 256;
-    s.rows = min(256, e.fresh * p.G - s.row0);
-    s.two = s.rows > 128;
-    s.slots = s.two || s.j1 - s.j0 > 1 ? 2u : 1u;
-    tile = 0;
-    ++hk;
-    return true;
+    return false;
   }
 };
 
@@ -310,6 +320,7 @@ struct OpenBlock {
   int32_t owner;  // the CTA whose share has its first tile (-1: none)
   int32_t parts;  // shares
   int32_t first, hk, row0, rows;
+  int32_t each;   // parts that a share has of it
 };
 
 // The place of tile j's K and V among a segment's loads (n tiles).
@@ -320,17 +331,28 @@ __device__ __forceinline__ uint32_t v_order(bool two, int32_t j, int32_t n) {
   return static_cast<uint32_t>(two || j + 1 == n ? 2 * j + 1 : 2 * j + 2);
 }
 
+// log2 of the copies that a segment's row tile holds of its rows.
+__device__ __forceinline__ uint32_t tree_log_copies(const Segment& s) {
+  return s.two || s.rows > 64 ? 0u : s.rows > 32 ? 1u : 2u;
+}
+
+__device__ __forceinline__ uint64_t mask_word(const TreeParams& p, const TreeEntry& e, int32_t i,
+                                              int32_t w) {
+  return static_cast<uint64_t>(p.mask[static_cast<int64_t>(e.first + i) * p.mask_words + w]);
+}
+
 // Bits of the 32 keys from kb on that new token i of the segment's request sees.
+// (`word0` is the first word of its mask)
 __device__ __forceinline__ uint32_t seen_bits(const TreeParams& p, const TreeEntry& e, int32_t i,
-                                              int32_t kb) {
+                                              uint64_t word0, int32_t kb) {
   auto low = [](int32_t n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; };
   const int32_t r = kb - e.ctx;  // rank of the first key among the new ones
   if (p.mask == nullptr) return low(min(i + 1, e.fresh) - r);
   uint32_t bits = low(-r);  // older tokens
   if (r > -32) {
-    const int64_t* words = p.mask + static_cast<int64_t>(e.first + i) * p.mask_words;
     auto word = [&](int32_t w) {
-      return w >= 0 && w < p.mask_words ? static_cast<uint64_t>(words[w]) : 0ull;
+      if (w <= 0) return w == 0 ? word0 : 0ull;
+      return w < p.mask_words ? mask_word(p, e, i, w) : 0ull;
     };
     const int32_t w = r >> 6, sh = r & 63;  // arithmetic: word -1 holds ranks -64 .. -1
     uint64_t v = word(w) >> sh;
@@ -346,7 +368,7 @@ template <int D, typename T, typename OutT>
 __device__ __noinline__ void add_odd_cache_values(const TreeParams& p, const Segment& s, int32_t i,
                                                   int32_t d0, int32_t n, OutT* out) {
   for (int32_t kb = s.j0 * 128; kb < min(s.j1 * 128, s.e.len); kb += 32) {
-    uint32_t bits = seen_bits(p, s.e, i, kb);
+    uint32_t bits = seen_bits(p, s.e, i, p.mask != nullptr ? mask_word(p, s.e, i, 0) : 0ull, kb);
     while (bits != 0u) {
       const int32_t key = kb + __ffs(static_cast<int>(bits)) - 1;
       bits &= bits - 1u;
@@ -363,39 +385,49 @@ __device__ __noinline__ void add_odd_cache_values(const TreeParams& p, const Seg
   }
 }
 
+__device__ __forceinline__ void softmax_warps_meet() {
+  asm volatile("bar.sync 1, 256;" ::: "memory");
+}
+
 // Joins share k of a block: a lane to a row, E float4 columns by P parts at a time,
 // whose loads are all in flight together (with eight warps on the SM their latency
 // and that of the arithmetic between them is what bounds this, so what depends on
 // the row alone is done once). More than P parts go in rounds with a running
-// maximum. Indices past the end repeat the last one: every load is unconditional.
+// maximum. With many parts and fewer than eight runs of columns, warps split a run's parts
+// and the first of them adds up what they leave in shared memory (`sums`, six floats
+// by 32 lanes each). Indices past the end repeat the last one: every load is
+// unconditional. All warps meet the same number of times.
 template <int D, bool kBF16, int E, int P>
 __device__ __noinline__ void join_parts(const TreeParams& p, const OpenBlock& b, int32_t k,
-                                        int32_t warp8, int32_t lane) {
+                                        int32_t warp8, int32_t lane, float* sums) {
   using T = typename std::conditional<kBF16, __nv_bfloat16, __half>::type;
   constexpr int32_t kRuns = D / 4 / E;  // runs of E columns in a row
-  const int32_t all = (b.rows + 31) / 32 * kRuns;
-  const int32_t to = all * (k + 1) / b.parts;
-  const int32_t part_step = 2 * (D / 4) * p.part_rows;  // float4s between two CTAs' parts
-  for (int32_t u = all * k / b.parts + warp8; u < to; u += 8) {
+  const int32_t all = (b.rows + 31) / 32 * kRuns, parts = b.parts * b.each;
+  const int32_t from = all * k / b.parts, to = all * (k + 1) / b.parts;
+  const int32_t ls = E > 1 || parts <= 16 || to - from >= 8 ? 0 : to - from >= 4 ? 1 : to - from >= 2 ? 2 : 3;
+  const int32_t split = warp8 & ((1 << ls) - 1);  // of the run's parts, this warp's
+  const int32_t step = p.part_rows * (D / 4);      // float4s of a part
+  for (int32_t u0 = from; u0 < to; u0 += 8 >> ls) {
+    const int32_t u1 = u0 + (warp8 >> ls), u = min(u1, to - 1);
     const int32_t r0 = u / kRuns * 32 + lane, r = min(r0, b.rows - 1), v = u % kRuns * E;
-    // the owner's part lies one slot after the others'
-    const float2* ml = p.part_ml + 2 * b.owner * p.part_rows + r;
-    const float4* po = reinterpret_cast<const float4*>(p.part) + b.owner * part_step +
-                       v * p.part_rows + r;
+    const float2* ml = p.part_ml + 4 * b.owner * p.part_rows + r;
+    const float4* po = reinterpret_cast<const float4*>(p.part) + 4 * b.owner * step + v * p.part_rows + r;
     float m = -INFINITY, l = 0.0f;
     float4 sum[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int32_t c0 = 0; c0 < b.parts; c0 += P) {
+    for (int32_t c0 = split; c0 < parts; c0 += P << ls) {
       float2 x[P];
       float4 o[P][E];
 #pragma unroll
       for (int c = 0; c < P; ++c) {
-        const int32_t part = min(c0 + c, b.parts - 1), first = part == 0 ? 1 : 0;
-        x[c] = __ldcg(ml + (2 * part + first) * p.part_rows);
+        const int32_t i = min(c0 + (c << ls), parts - 1);
+        const int32_t share = b.each == 2 ? i >> 1 : i;
+        // the owner's part lies in its second pair of slots, the others' in their first
+        const int32_t id = 4 * share + (share == 0 ? 2 : 0) + (b.each == 2 ? i & 1 : 0);
+        x[c] = __ldcg(ml + id * p.part_rows);
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          o[c][e] = __ldcg(po + part * part_step + (first * (D / 4) + e) * p.part_rows);
+        for (int e = 0; e < E; ++e) o[c][e] = __ldcg(po + id * step + e * p.part_rows);
       }
       float top = m;
 #pragma unroll
@@ -409,7 +441,8 @@ __device__ __noinline__ void join_parts(const TreeParams& p, const OpenBlock& b,
         sum[e] = make_float4(sum[e].x * was, sum[e].y * was, sum[e].z * was, sum[e].w * was);
 #pragma unroll
       for (int c = 0; c < P; ++c) {
-        if (c0 + c >= b.parts) continue;
+        // a part without anything may never have been written
+        if (c0 + (c << ls) >= parts || x[c].x == -INFINITY) continue;
         const float f = fast_exp2(x[c].x - top);
         l = fmaf(x[c].y, f, l);
 #pragma unroll
@@ -421,14 +454,49 @@ __device__ __noinline__ void join_parts(const TreeParams& p, const OpenBlock& b,
         }
       }
     }
-    if (r0 >= b.rows) continue;
+    if (E == 1 && ls > 0) {
+      float* mine = sums + warp8 * 6 * 32 + lane;
+      mine[0] = m;
+      mine[32] = l;
+      mine[64] = sum[0].x;
+      mine[96] = sum[0].y;
+      mine[128] = sum[0].z;
+      mine[160] = sum[0].w;
+      softmax_warps_meet();
+      if (split == 0) {
+        float top = -INFINITY;
+        for (int c = 0; c < (1 << ls); ++c) top = fmaxf(top, mine[c * 192]);
+        m = top;
+        l = 0.0f;
+        sum[0] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; top > -INFINITY && c < (1 << ls); ++c) {
+          const float* x = mine + c * 192;
+          const float f = fast_exp2(x[0] - top);
+          l = fmaf(x[32], f, l);
+          sum[0].x = fmaf(x[64], f, sum[0].x);
+          sum[0].y = fmaf(x[96], f, sum[0].y);
+          sum[0].z = fmaf(x[128], f, sum[0].z);
+          sum[0].w = fmaf(x[160], f, sum[0].w);
+        }
+      }
+      softmax_warps_meet();
+    }
+    if (split != 0 || u1 >= to || r0 >= b.rows) continue;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const int32_t g = b.row0 + r, t = g / p.G, h = b.hk * p.G + g - t * p.G;
     T* dst = static_cast<T*>(p.O) + static_cast<int64_t>(b.first + t) * p.o_t + h * p.o_h + 4 * v;
+    uint2 out[E];
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      reinterpret_cast<uint2*>(dst)[e] = make_uint2(pack2<kBF16>(sum[e].x * inv, sum[e].y * inv),
-                                                    pack2<kBF16>(sum[e].z * inv, sum[e].w * inv));
+      out[e] = make_uint2(pack2<kBF16>(sum[e].x * inv, sum[e].y * inv),
+                          pack2<kBF16>(sum[e].z * inv, sum[e].w * inv));
+    if constexpr (E == 1) {
+      *reinterpret_cast<uint2*>(dst) = out[0];
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; e += 2)
+        reinterpret_cast<uint4*>(dst)[e / 2] = make_uint4(out[e].x, out[e].y, out[e + 1].x, out[e + 1].y);
+    }
     if (v == 0 && p.lse != nullptr)
       p.lse[static_cast<int64_t>(h) * p.tokens + b.first + t] =
           l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.693147180559945309f;
@@ -665,7 +733,8 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
     }
   } else {
     // ------------------------------------ Q, softmax, epilogue and the join --
-    const uint32_t t = (warp - 2u) >> 2;       // warpgroup
+    const uint32_t w8 = warp - TP::kFirstSoftmax;
+    const uint32_t t = w8 >> 2;                // warpgroup
     const uint32_t quarter = warp & 3u;        // TMEM lane quarter of the warp
     const uint32_t row = quarter * 32u + lane;
     const uint32_t taddr = tmem_base + ((quarter * 32u) << 16);
@@ -683,13 +752,13 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
       if (alive && __all_sync(0xffffffffu, fmha_wait(bar, parity & 1u, abort_flag, p, site)) == 0)
         alive = false;
     };
-    auto meet = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+    auto meet = [&]() { softmax_warps_meet(); };
     // blocks of this share that other shares hold parts of: the first and the last
     OpenBlock open_first = {-1}, open_last = {-1};
 
     while (walk.next(p, w)) {
       const bool whole = w.j0 == 0 && w.j1 == w.e.tiles;
-      const uint32_t lc = w.two || w.rows > 64 ? 0u : w.rows > 32 ? 1u : 2u;
+      const uint32_t lc = tree_log_copies(w);
       const uint32_t copies = 1u << lc, per = 4u >> lc;  // copies of the rows, warps of a copy
       const uint32_t copy = quarter >> (2u - lc);
       const int32_t lrow = static_cast<int32_t>((quarter & (per - 1u)) * 32u + lane);  // row in the tile
@@ -725,10 +794,12 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
         if (lane == 0) mbar_arrive(q_full);
       }
 
-      float m_run = -INFINITY, l_run = 0.0f;
+      // the lanes without a row stay quiet: their maximum never moves
+      float m_run = real ? -INFINITY : INFINITY, l_run = 0.0f;
       uint32_t odd = 0;
       const int32_t n = w.j1 - w.j0;
       const int32_t stride = w.two ? 1 : 2;
+      const uint64_t word0 = p.mask != nullptr && real ? mask_word(p, w.e, tok, 0) : 0ull;
       for (int32_t j = w.two ? 0 : static_cast<int32_t>(t); j < n; j += stride, ++step) {
         const int32_t kb = (w.j0 + j) * 128;
         const bool masked = kb + 128 > w.e.ctx;  // some row may not see some key
@@ -753,7 +824,7 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
 #pragma unroll
           for (uint32_t c = 0; c < 4; ++c)
             if (c < per)
-              seen[c] = seen_bits(p, w.e, tok, kb + 32 * static_cast<int32_t>(c0 + c));
+              seen[c] = seen_bits(p, w.e, tok, word0, kb + 32 * static_cast<int32_t>(c0 + c));
         }
         if (per == 4u)
           tile_softmax<D, kBF16, 4>(s_col, o_col, 0u, p.scale_log2, masked, seen, first, m_run,
@@ -773,7 +844,9 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
         ++ti;
       }
       // where the rows go: O, or this share's unfinished rows
-      const int32_t part_id = 2 * me + (w.j0 == 0 ? 1 : 0);
+      const bool direct = w.two || (!whole && copies == 1u);  // no join in this CTA
+      const int32_t part_id =
+          4 * me + (w.j0 == 0 ? 2 : 0) + (direct && !w.two ? static_cast<int32_t>(t) : 0);
       float4* part = reinterpret_cast<float4*>(p.part) +
                      static_cast<int64_t>(part_id) * p.part_rows * (D / 4);
       float2* part_ml = p.part_ml + static_cast<int64_t>(part_id) * p.part_rows;
@@ -786,7 +859,9 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
               l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
         }
       };
-      if (w.two) {
+      if (direct && !active) {
+        if (real) store_sums(m_run, l_run);  // a sum of nothing: its O is never read
+      } else if (direct) {
         uint32_t o[D];
 #pragma unroll
         for (uint32_t d = 0; d < static_cast<uint32_t>(D); d += 32u)
@@ -795,7 +870,8 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(o_free(t));
-        const volatile uint32_t* m = odd_words + (ic & 1u) * 8u;
+        // two row tiles of one V: the first warpgroup looked; else each at its own
+        const volatile uint32_t* m = odd_words + (ic & 1u) * 8u + (w.two ? 0u : t * 4u);
         const bool any_odd = (m[0] | m[1] | m[2] | m[3]) != 0u;
         if (real) {
           store_sums(m_run, l_run);
@@ -906,7 +982,7 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
             return sum;
           };
           if (whole) {
-            for (uint32_t i = threadIdx.x - 64u; i < static_cast<uint32_t>(w.rows) << lv; i += 256u) {
+            for (uint32_t i = (threadIdx.x - 32u * TP::kFirstSoftmax); i < static_cast<uint32_t>(w.rows) << lv; i += 256u) {
               const uint32_t r = i >> lv, v = i & (vecs - 1u);
               const float4 sum = sum_of(r, v);
               const int32_t g = w.row0 + static_cast<int32_t>(r), tk = g / p.G;
@@ -918,7 +994,7 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
               if (any_odd) add_odd_cache_values<D, T>(p, w, tk, col, 4, dst);
             }
           } else {
-            for (uint32_t v = warp - 2u; v < vecs; v += 8u) {
+            for (uint32_t v = w8; v < vecs; v += 8u) {
               for (uint32_t r = lane; r < static_cast<uint32_t>(w.rows); r += 32u) {
                 const int32_t col = static_cast<int32_t>(d + 4u * v);
                 float4* dst = part + (col / 4) * p.part_rows + r;
@@ -940,6 +1016,7 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
         b.hk = w.hk;
         b.row0 = w.row0;
         b.rows = w.rows;
+        b.each = direct && !w.two ? 2 : 1;
         (w.j1 == w.e.tiles ? open_first : open_last) = b;
       }
       base += 2u * static_cast<uint32_t>(n);
@@ -952,7 +1029,7 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
     if (open_first.owner >= 0 || open_last.owner >= 0) {
       meet();
       const int32_t owner = lane == 0 ? open_first.owner : open_last.owner;
-      if (warp == 2u && lane < 2u && owner >= 0) {
+      if (w8 == 0u && lane < 2u && owner >= 0) {
         __threadfence();
         atomicAdd(&p.counters[2 * owner], 1u);
       }
@@ -961,7 +1038,7 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
     for (int slot = 0; slot < 2; ++slot) {
       const OpenBlock b = slot == 0 ? open_first : open_last;
       if (b.owner < 0) continue;
-      if (warp == 2u && lane == 0) {
+      if (w8 == 0u && lane == 0) {
         uint32_t* count = p.counters + 2 * b.owner;
         const uint64_t t0 = globaltimer_ns();
         bool there = true;
@@ -982,13 +1059,15 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
       }
       meet();
       if (*abort_flag != 0u) continue;
-      const int32_t k = me - b.owner, w8 = static_cast<int32_t>(warp) - 2, ln = static_cast<int32_t>(lane);
-      if (b.parts <= 2)
-        join_parts<D, kBF16, 4, 2>(p, b, k, w8, ln);
-      else if (b.parts <= 4)
-        join_parts<D, kBF16, 2, 4>(p, b, k, w8, ln);
+      const int32_t k = me - b.owner, wi = static_cast<int32_t>(w8), ln = static_cast<int32_t>(lane);
+      float* sums = reinterpret_cast<float*>(smem + TP::kJoinOff);
+      const int32_t parts = b.parts * b.each;
+      if (parts <= 2)
+        join_parts<D, kBF16, 4, 2>(p, b, k, wi, ln, sums);
+      else if (parts <= 4)
+        join_parts<D, kBF16, 2, 4>(p, b, k, wi, ln, sums);
       else
-        join_parts<D, kBF16, 1, 12>(p, b, k, w8, ln);
+        join_parts<D, kBF16, 1, 8>(p, b, k, wi, ln, sums);
     }
   }
 
@@ -1013,8 +1092,8 @@ TreeWorkspace tree_workspace(int64_t tokens, int group, int head_dim, int sms) {
   auto up = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
   w.part_rows = static_cast<int32_t>(std::min<int64_t>(256, tokens * group));
   w.part_ml = workspace_flag_bytes(sms);
-  w.part = w.part_ml + up(sizeof(float2) * 2 * static_cast<size_t>(sms) * w.part_rows);
-  w.total = w.part + sizeof(float) * 2 * static_cast<size_t>(sms) * w.part_rows * head_dim;
+  w.part = w.part_ml + up(sizeof(float2) * 4 * static_cast<size_t>(sms) * w.part_rows);
+  w.total = w.part + sizeof(float) * 4 * static_cast<size_t>(sms) * w.part_rows * head_dim;
   return w;
 }
 

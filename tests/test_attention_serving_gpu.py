@@ -522,3 +522,25 @@ def test_a_step_of_serving(cuda_device):
         size = v.float().abs().max()
         assert float(diff.max()) <= 4 * 2.0 ** -8 * float(size)
         assert at[-1] == sum(whole)
+
+
+def test_graph_outlives_a_larger_call(cuda_device):
+    """A captured call keeps its workspace when a larger one on the same stream needs more."""
+    small, big = (Tree(n, new, 8, 2, 128, 16, torch.bfloat16, seed=17) for n, new in
+                  (([3000], [1]), ([500] * 9, [40] * 9)))
+    side = torch.cuda.Stream()  # a stream that has no workspace yet
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want, _ = small.run()
+        lens, cu, o = torch.tensor(small.lens, dtype=torch.int32, device="cuda"), _cu([1]), torch.empty_like(small.q)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            attention.attention_tree(small.q, small.kc, small.vc, small.table, lens, cu, small.mask, o)
+        before = ops.workspace(0, side.device)
+        big.run()
+        assert ops.workspace(0, side.device) is not before and any(x is before for x in ops._outgrown)
+        torch.cuda.empty_cache()
+        graph.replay()
+    torch.cuda.current_stream().wait_stream(side)
+    ops.check_status()
+    assert torch.equal(o, want)
