@@ -9,19 +9,27 @@
 //   - kHeads: the same 128 rows of two query heads. With an even number of query
 //     heads per key/value head they share K and V, and both end with the same tile,
 //     so neither waits for the other and a prompt's ragged end leaves none idle.
-//     (With two row tiles of one head, as below, the first ends a tile earlier: 24
-//     uneven prompts took 157 us so, and 1.14 ms a prompt of 12031.)
 //   - kRows: two 128-row tiles of one head, for an odd number of heads per
-//     key/value head, where neighbouring heads would need two tiles of K and V.
+//     key/value head, where neighbouring heads would need two tiles of K and V (one
+//     prompt of 12031 tokens, 24 heads of 128 not grouped: 860 us so, 1199 with two
+//     heads and their own K and V each).
 //   - with an odd number, blocks of up to 128 rows are kHeads items too, whose heads
 //     may then differ in K and V: every KV tile takes two ring stages.
 // The blocks are listed in order of falling work and dealt to the CTAs in turns of
 // alternating direction, which evens out their sums. Up to kOwnBlocks of them every
-// CTA makes the list for itself (one prompt of 61 tokens: PLAN_OWN us on the GPU against
-// PLAN_KERNEL with a planning launch), above that a planning kernel does.
+// CTA makes the list for itself (one prompt of 61 tokens: 8.3 us on the GPU against 9.8
+// with a planning launch; 256 blocks are compared with one another in about as long as
+// the launch takes), above that a planning kernel does.
 //
 // What bounds it: the two products and the exponentials of a tile, as in
-// attention.cu, and for short prompts the hand-over from item to item.
+// attention.cu, and for short prompts the hand-over from item to item. 12031 tokens,
+// 32 heads over 8, 128: 945-1078 us (1250-1100 TFLOPS; the power cap moves it, 1689 is
+// the measured rate of a plain product); 24 prompts of 1 to 1100 tokens 129-145 us; 96
+// of up to 300, 24 heads of 64: 74-76 us (1.75 TB/s of what has to move). Measured and
+// not kept: half of a row's columns to each of two threads (16 softmax warps) 1213-1341
+// us for the first; one wait for all of P instead of one for each half, 5-8 % slower; a
+// quarter of the exponentials as poly_exp2, no gain at 128 and 9 % at 64, for a sum of
+// weights that is right to 1e-5 only.
 //
 // What is masked must not count whatever it holds, and 0 * NaN would: the keys of
 // the last KV tile may be another prompt's, or later tokens of the same one. So

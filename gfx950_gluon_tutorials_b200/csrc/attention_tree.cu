@@ -32,6 +32,12 @@
 // with its own maximum, sum and O; they meet in shared memory at the end of the
 // block, together with the two warpgroups'.
 //
+// Measured: 64 requests of up to 8192 keys, 32 heads over 8, one token each: 288-303 us,
+// 5.5-5.7 TB/s; 16 requests of up to 5000 keys with trees of up to 64 drafts 116 us; two
+// of 100003 and 81102 keys with up to 12 drafts, 16 heads over 2, 67.5 us; one of 777
+// keys, one token, 16.7 us. Pages of 16 tokens cost the decode a fifth (2 KB boxes). A
+// warp that fetches the next block's Q during the joins changed nothing.
+//
 // Pages: a tile is gathered by one TMA box per page and 64-element slab (a page
 // of 128 tokens or more is one box), each lane of the producer warp issuing one.
 // Keys past the request's length are loaded from past the last page, which fills

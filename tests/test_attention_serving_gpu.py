@@ -544,3 +544,16 @@ def test_graph_outlives_a_larger_call(cuda_device):
     torch.cuda.current_stream().wait_stream(side)
     ops.check_status()
     assert torch.equal(o, want)
+
+
+def test_example_serves(cuda_device):
+    """The example's last tokens equal a prefill of the accepted sequences up to two roundings
+    of the weights and of the output, and the projections' own (values of a few units)."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(__file__), "..", "examples", "serve_step.py")
+    spec = importlib.util.spec_from_file_location("serve_step", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    assert example.main() <= 4 * 2.0 ** -8 * 6.0  # 6: above any of the normal values of V
