@@ -82,7 +82,8 @@ struct PrefillPlan {
   static constexpr uint32_t kOddOff = kMiscOff + 16;            // [3][2 items][4 warps], see odd_words
   // a CTA's own list: int4 sorted[kOwnBlocks], unsorted[kOwnBlocks], int32 keys[kOwnBlocks]
   static constexpr uint32_t kListOff = (kOddOff + 96 + 15) / 16 * 16;
-  static constexpr uint32_t kBytes = kListOff + kOwnBlocks * 36;
+  static constexpr uint32_t kStoreOff = (kListOff + kOwnBlocks * 36 + 127) / 128 * 128;
+  static constexpr uint32_t kBytes = kStoreOff + kSoftmaxWarps * 2048;  // [warps][32 rows][32 values]
   static constexpr uint32_t kDynBytes = kBytes + 1024;  // + alignment slack
   static constexpr uint32_t kS = 0, kO = 256, kTileCols = 128;  // TMEM columns, as in attention.cu
   static_assert(kDynBytes <= 232448, "shared memory");
@@ -564,10 +565,14 @@ __global__ void __launch_bounds__(PrefillPlan<D>::kThreads, 1)
     auto wait_all = [&](uint32_t bar, uint32_t parity, int site) {
       return __all_sync(0xffffffffu, fmha_wait(bar, parity & 1u, abort_flag, p, site)) != 0;
     };
-    while (alive && walk.next(p, own_list, counts, w)) {
+    bool have = walk.next(p, own_list, counts, w);
+    while (alive && have) {
       const uint32_t stage0 = base;
       base += w.stages();
-      if (t >= w.slots) continue;
+      if (t >= w.slots) {
+        have = walk.next(p, own_list, counts, w);
+        continue;
+      }
       const int32_t n = w.tiles(t);
       float m_run = -INFINITY, l_run = 0.0f;  // offset in log2 units, sum of weights
       for (int32_t j = 0; j < n; ++j, ++step) {
@@ -606,7 +611,12 @@ __global__ void __launch_bounds__(PrefillPlan<D>::kThreads, 1)
       if (!alive) break;
 
       // epilogue: O into registers, the columns released to the next item's first PV,
-      // then the scaled rows stored
+      // then the scaled rows stored. What the next item is gets worked out while the
+      // last PV runs.
+      const int32_t head = w.head_of(t), m0 = w.m0, row0 = w.row0(t);
+      const int32_t rows = w.rows - (row0 - m0);  // of this tile that there are
+      const uint32_t two = w.slots - 1u;
+      have = walk.next(p, own_list, counts, w);
       if (!wait_all(o_done(t), ti, B2G_SITE_ACC_FULL)) break;
       tc_fence_after();
       uint32_t o[D];
@@ -617,27 +627,49 @@ __global__ void __launch_bounds__(PrefillPlan<D>::kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_free(t));
-      const int32_t head = w.head_of(t), token = w.row0(t) + static_cast<int32_t>(row);
-      if (token - w.m0 < w.rows) {
-        const float inv_l = l_run == 0.0f ? 0.0f : 1.0f / l_run;
-        T* orow = static_cast<T*>(p.O) + static_cast<int64_t>(token) * p.o_t + head * p.o_h;
+      const float inv_l = l_run == 0.0f ? 0.0f : 1.0f / l_run;
+      // 32 columns at a time through shared memory, so that four lanes store 64
+      // neighbouring bytes of a row (a row per lane costs a memory transaction per lane
+      // and 16 bytes). 16-byte piece c of row r sits at piece c ^ (r / 2 % 4), which
+      // spreads eight rows and eight pieces alike over the banks.
+      const uint32_t stage = sbase + PP::kStoreOff + (warp - 2u) * 2048u;
+      const uint32_t srow = lane >> 2, sc = lane & 3u;  // of the first of four stores
+      T* dst = static_cast<T*>(p.O) + static_cast<int64_t>(row0 + static_cast<int32_t>(quarter * 32u + srow)) * p.o_t +
+               head * p.o_h + 8u * sc;
 #pragma unroll
-        for (int v = 0; v < D / 8; ++v) {
-          uint4 u;
-          uint32_t* uw = &u.x;
+      for (uint32_t d = 0; d < static_cast<uint32_t>(D); d += 32u) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            uw[i] = pack2<kBF16>(__uint_as_float(o[8 * v + 2 * i]) * inv_l,
-                                 __uint_as_float(o[8 * v + 2 * i + 1]) * inv_l);
-          reinterpret_cast<uint4*>(orow)[v] = u;
+        for (uint32_t c = 0; c < 4; ++c) {
+          uint32_t u[4];
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i)
+            u[i] = pack2<kBF16>(__uint_as_float(o[d + 8 * c + 2 * i]) * inv_l,
+                                __uint_as_float(o[d + 8 * c + 2 * i + 1]) * inv_l);
+          st_shared_v4(stage + lane * 64u + ((c ^ ((lane >> 1) & 3u)) << 4), u);
         }
+        __syncwarp();
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+          const uint32_t r = srow + 8u * i;
+          uint32_t u[4];
+          ld_shared_v4(stage + r * 64u + ((sc ^ ((r >> 1) & 3u)) << 4), u);
+          if (static_cast<int32_t>(quarter * 32u + r) < rows)
+            *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(8u * i) * p.o_t + d) =
+                make_uint4(u[0], u[1], u[2], u[3]);
+        }
+        __syncwarp();
+      }
+      if (static_cast<int32_t>(row) < rows) {
+        const int32_t token = row0 + static_cast<int32_t>(row);
         uint32_t any = 0;
 #pragma unroll
         for (uint32_t q = 0; q < 4; ++q) {
           any |= odd_words[(t * 2u + (ti & 1u)) * 4u + q];
           if (t == 1u) any |= odd_words[(4u + (pairs & 1u)) * 4u + q];
         }
-        if (any != 0u) add_odd_values<D>(p, w.m0, head / p.G, token + 1, orow);
+        if (any != 0u)  // (the warp's stores above are visible to it: __syncwarp)
+          add_odd_values<D>(p, m0, head / p.G, token + 1,
+                            static_cast<T*>(p.O) + static_cast<int64_t>(token) * p.o_t + head * p.o_h);
         if (p.lse != nullptr) {
           constexpr float kLn2 = 0.693147180559945309f;
           p.lse[static_cast<int64_t>(head) * p.tokens + token] =
@@ -645,7 +677,7 @@ __global__ void __launch_bounds__(PrefillPlan<D>::kThreads, 1)
         }
       }
       ++ti;
-      pairs += w.slots - 1u;
+      pairs += two;
     }
   }
 
