@@ -57,6 +57,7 @@ struct alignas(64) PrefillParams {
   const int4* plan;           // blocks: {first token, its row in the prompt, prompt's rows, 0}; null: own list
   const int2* counts;         // kRows blocks (first in the plan), kHeads blocks
   int32_t HQ, G, tokens, prompts, block;
+  uint32_t hq_inv, pairs_inv;  // 2^32 / HQ and / (head pairs), rounded up; 0: divide
   float scale_log2;
   uint64_t timeout_ns;
 };
@@ -274,6 +275,11 @@ struct PrefillItem {
   }
 };
 
+// n / d with inv = 2^32 / d rounded up, exact while n d < 2^32, or 0.
+__device__ __forceinline__ int32_t quotient(int32_t n, int32_t d, uint32_t inv) {
+  return inv != 0u ? static_cast<int32_t>(__umulhi(static_cast<uint32_t>(n), inv)) : n / d;
+}
+
 // Walks a CTA's items. What it needs of the list stays in shared memory or is
 // prefetched an item ahead: registers are the softmax's.
 struct PrefillWalk {
@@ -285,29 +291,33 @@ struct PrefillWalk {
     const int4* list = p.plan == nullptr ? own : p.plan;
     const int32_t pairs = (p.HQ + 1) / 2, row_blocks = counts->x, row_items = row_blocks * p.HQ;
     const int32_t items = row_items + counts->y * pairs;
-    auto entry = [&](int32_t i) { return i < row_items ? i / p.HQ : row_blocks + (i - row_items) / pairs; };
+    auto block_of = [&](int32_t i) {
+      return i < row_items ? quotient(i, p.HQ, p.hq_inv)
+                           : row_blocks + quotient(i - row_items, pairs, p.pairs_inv);
+    };
     if (item >= items) return false;
-    const int4 e = list[entry(item)];
+    const int32_t block = block_of(item);
+    const int4 e = list[block];
     w.by_rows = item < row_items;
     w.m0 = e.x;
     w.k0 = e.x - e.y;
     w.rows = e.z - e.y;
     if (w.by_rows) {
-      w.head = item % p.HQ;
+      w.head = item - block * p.HQ;
       w.slots = 2;
       w.shared = true;
       w.n = e.y / 128 + 2;
     } else {
-      w.head = 2 * ((item - row_items) % pairs);
+      w.head = 2 * (item - row_items - (block - row_blocks) * pairs);
       w.slots = w.head + 1 < p.HQ ? 2u : 1u;
-      w.shared = w.slots == 1u || w.head / p.G == (w.head + 1) / p.G;
+      w.shared = (p.G & 1) == 0 || w.slots == 1u || w.head / p.G == (w.head + 1) / p.G;
       w.n = e.y / 128 + 1;
     }
     const int32_t g = static_cast<int32_t>(gridDim.x), c = static_cast<int32_t>(blockIdx.x);
     item += (turn & 1u) ? 2 * c + 1 : 2 * (g - c) - 1;
     ++turn;
     if (p.plan != nullptr && item < items)
-      asm volatile("prefetch.global.L1 [%0];" ::"l"(p.plan + entry(item)));
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(p.plan + block_of(item)));
     return true;
   }
 };
@@ -813,6 +823,13 @@ extern "C" int b2g_attention_prefill(const void* q, const void* k, const void* v
   prm.HQ = heads_q;
   prm.G = group;
   prm.tokens = static_cast<int32_t>(tokens);
+  // every item number is below blocks * HQ
+  auto inverse = [&](int64_t d) {
+    const bool exact = d > 1 && blocks * heads_q * d < (static_cast<int64_t>(1) << 32);
+    return exact ? static_cast<uint32_t>(((static_cast<int64_t>(1) << 32) + d - 1) / d) : 0u;
+  };
+  prm.hq_inv = inverse(heads_q);
+  prm.pairs_inv = inverse((heads_q + 1) / 2);
   prm.scale_log2 = sm_scale * 1.4426950408889634f;
   prm.timeout_ns = wait_timeout_ns();
   const bool bf16 = dtype == B2G_DT_BF16;
