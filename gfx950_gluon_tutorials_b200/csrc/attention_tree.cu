@@ -92,6 +92,7 @@ struct alignas(64) TreeParams {
   int32_t mask_words, part_rows, requests;
   int32_t most;            // keys that a table has room for
   int32_t HQ, HK, G, tokens, page_size, num_pages;
+  int32_t inject;          // test hook: joins wait for a part that nobody publishes
   float scale_log2;
   uint64_t timeout_ns;
 };
@@ -1048,7 +1049,7 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
         uint32_t* count = p.counters + 2 * b.owner;
         const uint64_t t0 = globaltimer_ns();
         bool there = true;
-        while (ld_acquire_gpu(count) < static_cast<uint32_t>(b.parts)) {
+        while (ld_acquire_gpu(count) < static_cast<uint32_t>(b.parts + p.inject)) {
           if (*abort_flag != 0u || globaltimer_ns() - t0 > p.timeout_ns) {
             fmha_report(p, B2G_STATUS_TIMEOUT | B2G_SITE_FLAG);
             *abort_flag = 1u;
@@ -1138,9 +1139,19 @@ int launch_tree(const TreeParams& prm, int sms, cudaStream_t stream) {
     attr_set[dev].store(true);
   }
   // one CTA per SM: the CTAs that share a block wait for one another, so all of
-  // them have to be resident
-  kern<<<static_cast<unsigned>(sms), TP::kThreads, TP::kDynBytes, stream>>>(prm);
-  const cudaError_t e = cudaGetLastError();
+  // them have to be resident, which a cooperative launch guarantees
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(sms), 1, 1);
+  cfg.blockDim = dim3(TP::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = TP::kDynBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeCooperative;
+  attr[0].val.cooperative = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, prm);
+  if (e != cudaSuccess) cudaGetLastError();
   return e == cudaSuccess ? B2G_OK : static_cast<int>(e);
 }
 
@@ -1227,6 +1238,7 @@ extern "C" int b2g_attention_tree(const void* q, const void* k_cache, const void
   prm.num_pages = static_cast<int32_t>(num_pages);
   prm.scale_log2 = sm_scale * 1.4426950408889634f;
   prm.timeout_ns = wait_timeout_ns();
+  prm.inject = inject_flag_timeout() ? 1 : 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = dtype == B2G_DT_BF16;
   if (head_dim == 128)

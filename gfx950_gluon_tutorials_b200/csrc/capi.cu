@@ -696,6 +696,8 @@ int check_serving_attention(int heads_q, int heads_k, int head_dim, int dtype, f
 
 PFN_cuTensorMapEncodeTiled_v12000 tma_encoder() { return tensor_map_encoder(); }
 
+bool inject_flag_timeout() { return g_opt.inject.load() != 0; }
+
 uint64_t wait_timeout_ns() { return static_cast<uint64_t>(g_opt.timeout_ms.load()) * 1000000ull; }
 
 }  // namespace b2g

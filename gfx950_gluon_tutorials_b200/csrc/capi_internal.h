@@ -37,6 +37,9 @@ int check_serving_attention(int heads_q, int heads_k, int head_dim, int dtype, f
                             const int64_t* strides, int n,
                             std::initializer_list<const void*> pointers);
 
+// Whether B2G_OPT_INJECT_FLAG_TIMEOUT is set.
+bool inject_flag_timeout();
+
 // The bounded-wait limit (B2G_OPT_TIMEOUT_MS) in nanoseconds.
 uint64_t wait_timeout_ns();
 

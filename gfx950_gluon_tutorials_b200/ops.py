@@ -104,6 +104,9 @@ def check_status(device: torch.device | None = None, reset: bool = True) -> None
             for (idx, _), ws in _workspaces.items():
                 if idx == device.index:
                     ws.zero_()
+            for ws in _outgrown:
+                if ws.get_device() == device.index:
+                    ws.zero_()
         if reset:
             st.zero_()
         torch.cuda.synchronize(device)

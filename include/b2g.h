@@ -374,9 +374,10 @@ B2G_API int b2g_cast_e5m2(const void* src, int src_dtype, int64_t n, uint8_t* ds
 #define B2G_OPT_MIN_SK_ITERS 4 /* minimum k-iterations (256-byte stages) per stream-K unit
                                   or split piece (default 16) */
 #define B2G_OPT_TIMEOUT_MS 5  /* bounded-wait deadline in ms (default 2000) */
-#define B2G_OPT_INJECT_FLAG_TIMEOUT 6 /* test hook: stream-K owners wait for a flag
-                                         value no contributor writes, so the wait
-                                         expires and the status word is set */
+#define B2G_OPT_INJECT_FLAG_TIMEOUT 6 /* test hook: stream-K owners (and the joins of
+                                         b2g_attention_tree) wait for a flag value no
+                                         contributor writes, so the wait expires and
+                                         the status word is set */
 #define B2G_OPT_MAX_UNITS 7   /* cap on persistent work units (0 = one per SM / pair) */
 #define B2G_OPT_L2_PREFETCH 8 /* k-iterations of A/B the producer pulls into L2 ahead
                                  of its shared-memory loads (default 0 = off) */

@@ -557,3 +557,23 @@ def test_example_serves(cuda_device):
     example = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(example)
     assert example.main() <= 4 * 2.0 ** -8 * 6.0  # 6: above any of the normal values of V
+
+
+def test_tree_join_that_never_comes(cuda_device):
+    """Parts that nobody publishes: every wait runs out, the kernel ends with a status, and the
+    next call is right again."""
+    t = Tree([9000, 70], [3, 1], 8, 2, 128, 16, torch.bfloat16, seed=18)
+    want, _ = t.run()
+    limit = _lib.get_option(_lib.OPT_TIMEOUT_MS)
+    try:
+        _lib.set_option(_lib.OPT_TIMEOUT_MS, 20)
+        _lib.set_option(_lib.OPT_INJECT_FLAG_TIMEOUT, 1)
+        with pytest.raises(_lib.B2GError) as e:
+            t.run()
+        assert e.value.code == _lib.STATUS_TIMEOUT | _lib.SITE_FLAG
+    finally:
+        _lib.set_option(_lib.OPT_INJECT_FLAG_TIMEOUT, 0)
+        _lib.set_option(_lib.OPT_TIMEOUT_MS, limit)
+    o, lse = t.run()
+    t.check(o, lse)
+    assert torch.equal(o, want)
