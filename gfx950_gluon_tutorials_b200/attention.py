@@ -210,8 +210,10 @@ def _run_packed(call, nbytes, dev, q, o, lse, args) -> torch.Tensor:
     tensor if it is None) with the stream's workspace as it is; asks ``nbytes`` how large that has
     to be only when the call finds it too small."""
     if o is None:
-        o = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    out, o_token, o_head = _packed(o)  # a copy keeps the rows past the last sequence
+        out = o = q.new_empty(q.shape)
+        o_token, o_head, _ = o.stride()
+    else:
+        out, o_token, o_head = _packed(o)  # a copy keeps the rows past the last sequence
     args = args(out.data_ptr(), o_token, o_head, None if lse is None else lse.data_ptr())
     ws, status, stream = workspace(0, dev), status_tensor(dev).data_ptr(), _stream_handle(dev)
     rc = call(*args, ws.data_ptr(), ws.numel(), status, stream)

@@ -35,8 +35,12 @@
 // Measured: 64 requests of up to 8192 keys, 32 heads over 8, one token each: 288-303 us,
 // 5.5-5.7 TB/s; 16 requests of up to 5000 keys with trees of up to 64 drafts 116 us; two
 // of 100003 and 81102 keys with up to 12 drafts, 16 heads over 2, 67.5 us; one of 777
-// keys, one token, 16.7 us. Pages of 16 tokens cost the decode a fifth (2 KB boxes). A
-// warp that fetches the next block's Q during the joins changed nothing.
+// keys, one token, 16.7 us. Pages of 16 tokens cost the decode a fifth: a box of 2 KB
+// takes about 100 cycles to issue and there are 32 to a tile. Issued from one lane of a
+// converged warp they cost less (344 -> 313 us) but the few boxes of larger pages more
+// (288 -> 308), and code for both slowed either. Asking tiles into L2 ahead of the ring
+// adds boxes and lost 3-25 %. A warp that fetches the next block's Q during the joins
+// changed nothing.
 //
 // Pages: a tile is gathered by one TMA box per page and 64-element slab (a page
 // of 128 tokens or more is one box), each lane of the producer warp issuing one.
@@ -97,6 +101,8 @@ struct alignas(64) TreeParams {
   uint64_t timeout_ns;
 };
 
+// Tiles that beginning a block counts as in the cut of the shares. Interleaved, for 0 / 5 /
+// 8: 16 drafted trees 124-132 / 117 / 116 us, two long caches 72-76 / 72 / 68, decode alike.
 constexpr int32_t kBlockCost = 8;
 
 template <int D>

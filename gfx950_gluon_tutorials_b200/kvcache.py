@@ -89,9 +89,9 @@ def map_step(cached_lens: torch.Tensor, new_lens: torch.Tensor, page_counts: tor
         raise ValueError("page_size must be positive and num_tokens not negative")
     # one allocation for the int32 outputs
     n = num_tokens
-    slots = torch.empty(n, dtype=torch.int64, device=dev)
-    ints = torch.empty(n + 3 * requests + 2, dtype=i32, device=dev)
-    positions, cu, seq, counts, left = ints.split_with_sizes(
+    slots = block_tables.new_empty(n, dtype=torch.int64)
+    ints = block_tables.new_empty(n + 3 * requests + 2)
+    positions, cu, seq, counts, left = ints.unsafe_split_with_sizes(
         (n, requests + 1, requests, requests, 1))
     base = ints.data_ptr()
     rc = _lib.lib().b2g_kv_map_step(
