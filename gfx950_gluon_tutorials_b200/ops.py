@@ -67,8 +67,9 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     with _ws_lock:
         ws = _workspaces.get(key)
         if ws is None or ws.numel() < nbytes:
-            if ws is not None:
+            if ws is not None:  # by half at least, so that those kept add up to little
                 _outgrown.append(ws)
+                nbytes = max(nbytes, ws.numel() * 3 // 2)
             ws = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device)
             _workspaces[key] = ws
         return ws

@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes
 
+import numpy as np
 import pytest
 import torch
 
@@ -25,6 +26,30 @@ def test_oracle_by_hand():
     assert out["positions"] == [3, 4, 5, 6, 7, 8, 0, 0]
     assert out["cu_seqlens"] == [0, 6, 7] and out["seq_lens"] == [9, 1]
     assert out["page_counts"] == [3, 1] and out["num_free"] == [1]
+
+
+@pytest.mark.parametrize("unit", [2.0 ** -8, 2.0 ** -11])
+def test_oracle_attention(unit):
+    """The float64 restatement against a softmax written out, rows that see nothing, masked NaN,
+    and its tolerances against attention whose weights and output are rounded by ``unit``."""
+    rng = np.random.default_rng(3)
+    q, k, v = rng.standard_normal((5, 16)), rng.standard_normal((9, 16)), rng.standard_normal((9, 16))
+    seen = serving.tree_seen(9, 5, [1, 0b11, 0b101, 0b1011, 0b10011])
+    assert seen[:, :4].all() and seen[3, 4:].tolist() == [True, True, False, True, False]
+    assert (serving.tree_seen(9, 9) == serving.causal(9)).all()
+    seen[2] = False
+    k[8], v[8] = np.nan, np.inf  # the last draft is seen by the last row alone
+    o, lse, tol, lse_tol = serving.attend(q, k, v, seen, 0.25, unit)
+    assert (o[2] == 0).all() and lse[2] == -np.inf and not np.isfinite(o[4]).any()
+    for i in (0, 1, 3):
+        idx = np.flatnonzero(seen[i])
+        w = np.exp(0.25 * (k[idx] @ q[i]))
+        np.testing.assert_allclose(o[i], (w[:, None] * v[idx]).sum(0) / w.sum(), rtol=1e-12)
+        np.testing.assert_allclose(lse[i], np.log(w.sum()), rtol=1e-12)
+        w /= w.max()
+        rounded = w * (1 + unit * rng.choice([-1, 1], w.shape))
+        off = (rounded[:, None] * v[idx]).sum(0) / w.sum() * (1 + unit * rng.choice([-1, 1], 16))
+        assert (np.abs(off - o[i]) <= tol[i] * (1 + unit)).all() and lse_tol[i] > 0
 
 
 MAP = dict(cached=16, new=16, counts=16, tables=16, stride=8, requests=2, max_pages=8, free=16,
