@@ -577,3 +577,19 @@ def test_tree_join_that_never_comes(cuda_device):
     o, lse = t.run()
     t.check(o, lse)
     assert torch.equal(o, want)
+
+
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("new", [1, 12, 25, 70], ids=["four copies", "two copies", "one", "two row tiles"])
+def test_tree_odd_value_in_the_context(cuda_device, new, what):
+    """A value of an older token that is not finite comes out in its dim of every row, as itself,
+    and changes no other dim."""
+    t = Tree([900 + new], [new], 8, 2, 128, 16, torch.bfloat16, seed=19, masked=False)
+    want, _ = t.run()
+    page, slot = int(t.table[0, 517 // 16]), 517 % 16
+    t.vc[page, slot, :, 7] = what
+    o, _ = t.run()
+    got = o[..., 7].float()
+    assert bool(got.isnan().all() if math.isnan(what) else (got == what).all())
+    keep = torch.arange(128, device="cuda") != 7
+    assert torch.equal(o[..., keep], want[..., keep])
