@@ -212,6 +212,8 @@ __device__ __forceinline__ void find_share(const TreeParams& p, int64_t* sums, S
   }
   if (lane == 31u) sums[warp] = scan;
   if (lane == 0u) sums[kWarps + warp] = sum;
+  // before the barrier: the thread that finds the share stores its length after it
+  if (threadIdx.x == 0) out->here = 0;
   __syncthreads();
   int64_t total = 0, base = 0, upto = 0;
 #pragma unroll
@@ -224,10 +226,7 @@ __device__ __forceinline__ void find_share(const TreeParams& p, int64_t* sums, S
   const int64_t ctas = min(units, static_cast<int64_t>(gridDim.x));
   const int64_t u =
       ctas > 0 ? share_begin(units, static_cast<int32_t>(blockIdx.x), static_cast<int32_t>(ctas)) : 0;
-  if (threadIdx.x == 0) {
-    out->units = units;
-    out->here = 0;
-  }
+  if (threadIdx.x == 0) out->units = units;
   if (static_cast<int64_t>(blockIdx.x) >= ctas) return;
   int64_t n = first, before = base + scan - first;  // units a head of this thread's request, and before it
   for (int32_t r0 = 0;;) {
