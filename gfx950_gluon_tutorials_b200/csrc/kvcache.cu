@@ -47,6 +47,7 @@ struct MapStepParams {
 
 constexpr int kMapThreads = 512;
 constexpr int kMapMaxRequests = 8192;  // two int32 prefix sums per request in shared memory
+constexpr int kMapStaticBytes = 2 * (kMapThreads / 32) * 8;  // warp_tok and warp_pag
 
 __device__ __forceinline__ void report(int* status, int code) {
   if (status != nullptr) atomicCAS(status, 0, code);
@@ -67,6 +68,7 @@ __global__ void __launch_bounds__(kMapThreads) map_step_kernel(const MapStepPara
   extern __shared__ int32_t ends[];  // [requests] token ends, then [requests] page ends
   int32_t* page_ends = ends + p.requests;
   __shared__ int64_t warp_tok[kMapThreads / 32], warp_pag[kMapThreads / 32];
+  static_assert(sizeof(warp_tok) + sizeof(warp_pag) == kMapStaticBytes, "static shared memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t limit = p.num_tokens;
   int64_t tok_base = 0, pag_base = 0;  // sums over the chunks before this one (same in all threads)
@@ -284,7 +286,8 @@ extern "C" int b2g_kv_map_step(const int32_t* cached_lens, const int32_t* new_le
   p.page_size = page_size;
   p.num_tokens = static_cast<int32_t>(num_tokens);
   const int smem = std::max(requests, 1) * 2 * static_cast<int>(sizeof(int32_t));
-  if (smem > 48 * 1024) {
+  // what a launch may take unasked (48 KB) holds the kernel's static arrays too
+  if (smem + kMapStaticBytes > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(
         map_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
         kMapMaxRequests * 2 * static_cast<int>(sizeof(int32_t)));
