@@ -408,7 +408,9 @@ __device__ __forceinline__ void softmax_warps_meet() {
 // maximum. With many parts and fewer than eight runs of columns, warps split a run's parts
 // and the first of them adds up what they leave in shared memory (`sums`, six floats
 // by 32 lanes each). Indices past the end repeat the last one: every load is
-// unconditional. All warps meet the same number of times.
+// unconditional. All warps meet the same number of times. A part without anything is
+// one whose sum is zero: scores that are all NaN leave a maximum of -inf too, and have
+// to come out as NaN.
 template <int D, bool kBF16, int E, int P>
 __device__ __noinline__ void join_parts(const TreeParams& p, const OpenBlock& b, int32_t k,
                                         int32_t warp8, int32_t lane, float* sums) {
@@ -444,8 +446,8 @@ __device__ __noinline__ void join_parts(const TreeParams& p, const OpenBlock& b,
       float top = m;
 #pragma unroll
       for (int c = 0; c < P; ++c) top = fmaxf(top, x[c].x);
-      if (top == -INFINITY) continue;  // the row has seen nothing so far
-      const float was = fast_exp2(m - top);
+      const float ref = top == -INFINITY ? 0.0f : top;  // nothing so far, or only NaN
+      const float was = fast_exp2(m - ref);
       m = top;
       l *= was;
 #pragma unroll
@@ -454,8 +456,8 @@ __device__ __noinline__ void join_parts(const TreeParams& p, const OpenBlock& b,
 #pragma unroll
       for (int c = 0; c < P; ++c) {
         // a part without anything may never have been written
-        if (c0 + (c << ls) >= parts || x[c].x == -INFINITY) continue;
-        const float f = fast_exp2(x[c].x - top);
+        if (c0 + (c << ls) >= parts || x[c].y == 0.0f) continue;
+        const float f = fast_exp2(x[c].x - ref);
         l = fmaf(x[c].y, f, l);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -478,12 +480,13 @@ __device__ __noinline__ void join_parts(const TreeParams& p, const OpenBlock& b,
       if (split == 0) {
         float top = -INFINITY;
         for (int c = 0; c < (1 << ls); ++c) top = fmaxf(top, mine[c * 192]);
+        const float ref = top == -INFINITY ? 0.0f : top;
         m = top;
         l = 0.0f;
         sum[0] = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int c = 0; top > -INFINITY && c < (1 << ls); ++c) {
+        for (int c = 0; c < (1 << ls); ++c) {
           const float* x = mine + c * 192;
-          const float f = fast_exp2(x[0] - top);
+          const float f = fast_exp2(x[0] - ref);
           l = fmaf(x[32], f, l);
           sum[0].x = fmaf(x[64], f, sum[0].x);
           sum[0].y = fmaf(x[96], f, sum[0].y);
@@ -925,7 +928,8 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
         auto warp_of = [&](uint32_t c, uint32_t r) {
           return ((c >> lc) << 2) + ((c & (copies - 1u)) << (2u - lc)) + (r >> 5);
         };
-        float m_tot = -INFINITY, l_tot = 0.0f;
+        // (a maximum of -inf: nothing seen, with sums of zero, or only NaN, with sums of NaN)
+        float m_tot = -INFINITY, l_tot = 0.0f, ref;
         {
           float2 x[8];
 #pragma unroll
@@ -934,11 +938,11 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
                              : make_float2(-INFINITY, 0.0f);
 #pragma unroll
           for (uint32_t c = 0; c < 8; ++c) m_tot = fmaxf(m_tot, x[c].x);
-          if (m_tot > -INFINITY)
+          ref = m_tot == -INFINITY ? 0.0f : m_tot;
 #pragma unroll
-            for (uint32_t c = 0; c < 8; ++c) l_tot = fmaf(x[c].y, fast_exp2(x[c].x - m_tot), l_tot);
+          for (uint32_t c = 0; c < 8; ++c) l_tot = fmaf(x[c].y, fast_exp2(x[c].x - ref), l_tot);
         }
-        float scale = m_tot > -INFINITY ? fast_exp2(m_run - m_tot) : 0.0f;
+        float scale = fast_exp2(m_run - ref);
         if (whole) scale = l_tot == 0.0f ? 0.0f : scale / l_tot;
         if (t == 0u && copy == 0u && real) store_sums(m_tot, l_tot);
         // A round takes 32 columns, or as many as the buffer holds of fewer rows: it
