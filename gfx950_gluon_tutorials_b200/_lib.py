@@ -39,6 +39,7 @@ SIGNATURES = {
     "b2g_strerror": (ctypes.c_char_p, [_c_int]),
     "b2g_gemm_workspace_bytes": (_c_sz, [_c_int, _c_int, _c_int, _c_int]),
     "b2g_workspace_reset": (_c_int, [_vp, _c_sz, _vp]),
+    "b2g_exchange_capture_mode": (_c_int, [ctypes.POINTER(_c_int)]),
     "b2g_gemm_f16": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_int, _c_int, _c_int,
                               _c_int, _c_int, _vp, _c_sz, _vp, _vp]),
     "b2g_gemm_f8": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64,

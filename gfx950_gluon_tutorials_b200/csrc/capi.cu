@@ -766,6 +766,15 @@ int b2g_workspace_reset(void* workspace, size_t bytes, void* stream) {
   return e == cudaSuccess ? B2G_OK : static_cast<int>(e);
 }
 
+int b2g_exchange_capture_mode(int* mode) {
+  if (mode == nullptr || *mode < 0 || *mode > 2) return B2G_EINVAL;
+  cudaStreamCaptureMode m = static_cast<cudaStreamCaptureMode>(*mode);
+  const cudaError_t e = cudaThreadExchangeStreamCaptureMode(&m);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  *mode = static_cast<int>(m);
+  return B2G_OK;
+}
+
 int b2g_gemm_f16(const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int64_t ldc,
                  int M, int N, int K, int in_dtype, int out_dtype, void* workspace,
                  size_t workspace_bytes, int* status, void* stream) {

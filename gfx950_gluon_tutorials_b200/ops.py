@@ -55,10 +55,38 @@ def _require_cuda(*ts: torch.Tensor) -> torch.device:
     return dev
 
 
+def _zeros(n: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """``torch.zeros`` whose zeros are there while the current stream is being captured too.
+
+    A memset on a captured stream belongs to the graph: it runs at every replay of that
+    graph and not before the first, and the memory is the graph's. So there the tensor is
+    made, cleared and waited for on a stream that is not captured."""
+    with torch.cuda.device(device):
+        if not torch.cuda.is_current_stream_capturing():
+            return torch.zeros(n, dtype=dtype, device=device)
+        mode = ctypes.c_int(2)  # relaxed: cudaMalloc is allowed during the capture
+        check(lib().b2g_exchange_capture_mode(ctypes.byref(mode)), "b2g_exchange_capture_mode")
+        try:
+            for _ in range(64):  # torch hands out its streams in turn, captured ones too
+                side = torch.cuda.Stream(device)
+                with torch.cuda.stream(side):
+                    if torch.cuda.is_current_stream_capturing():
+                        continue
+                    t = torch.empty(n, dtype=dtype, device=device).zero_()
+                side.synchronize()
+                return t
+        finally:
+            lib().b2g_exchange_capture_mode(ctypes.byref(mode))
+    raise RuntimeError("no stream outside the capture to clear a workspace on: make one call "
+                       "before capturing")
+
+
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     """Zero-initialised scratch of at least ``nbytes`` for (device, current stream).
 
-    The kernels leave it zeroed after a successful run, so it is reused as is.
+    The kernels leave it zeroed after a successful run, so it is reused as is: by later
+    calls on the stream and by CUDA graphs captured on it, none of which may overlap on the
+    GPU (graphs that are replayed side by side are captured on streams of their own).
     """
     key = (device.index, _stream_handle(device))
     ws = _workspaces.get(key)
@@ -70,7 +98,7 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
             if ws is not None:  # by half at least, so that those kept add up to little
                 _outgrown.append(ws)
                 nbytes = max(nbytes, ws.numel() * 3 // 2)
-            ws = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device)
+            ws = _zeros(max(nbytes, 256), torch.uint8, device)
             _workspaces[key] = ws
         return ws
 
@@ -83,7 +111,7 @@ def status_tensor(device: torch.device) -> torch.Tensor:
     with _ws_lock:
         st = _status.get(device.index)
         if st is None:
-            st = torch.zeros(1, dtype=torch.int32, device=device)
+            st = _zeros(1, torch.int32, device)
             _status[device.index] = st
         return st
 
@@ -428,8 +456,8 @@ class PreparedGemm:
         self.device, self.c = dev, c
         self._keep = (a_, b_, c) + keep
         # a zeroed workspace of its own (its flag words must read zero at rest)
-        self._ws = torch.zeros(max(lib().b2g_gemm_workspace_bytes(kind, M, N, K), 256),
-                               dtype=torch.uint8, device=dev)
+        self._ws = _zeros(max(lib().b2g_gemm_workspace_bytes(kind, M, N, K), 256), torch.uint8,
+                          dev)
         self._h = ctypes.c_void_p()
         rc = lib().b2g_prepare_gemm(kind, a_.data_ptr(), a_.stride(0), b_.data_ptr(),
                                     b_.stride(0), *sa, *sb, c.data_ptr(), c.stride(0), M, N, K,

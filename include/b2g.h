@@ -102,6 +102,12 @@ B2G_API size_t b2g_gemm_workspace_bytes(int kind, int M, int N, int K);
  * nonzero status). */
 B2G_API int b2g_workspace_reset(void* workspace, size_t bytes, void* stream);
 
+/* Swaps *mode with this thread's stream capture mode (a cudaStreamCaptureMode: 0
+ * global, 1 thread-local, 2 relaxed). Under "relaxed" a thread may allocate and
+ * clear a workspace on another stream while it captures one into a CUDA graph;
+ * memory cleared on the captured stream is not clear until the graph runs. */
+B2G_API int b2g_exchange_capture_mode(int* mode);
+
 /* a16w16: C = A * B^T, A/B fp16 or bf16 (`in_dtype`), C fp16 or bf16
  * (`out_dtype`). lda, ldb and ldc must be multiples of 8 elements (16-byte
  * rows); K itself is free. */

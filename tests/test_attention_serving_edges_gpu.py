@@ -4,10 +4,15 @@ batches large enough for every way of planning the work. Against float64, as the
 
 from __future__ import annotations
 
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
-from test_attention_serving_gpu import DTYPES, Tree
+from gfx950_gluon_tutorials_b200 import attention, ops
+from test_attention_serving_gpu import DTYPES, Tree, _cu
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +59,93 @@ def test_tree_keys_of_nan_fill_a_share(cuda_device, new):
     t.kc[t.table[0].long()[at // 16], at % 16] = float("nan")
     o, lse = t.run()
     assert bool(o.isnan().all()) and bool(lse.isnan().all())
+
+
+def _fresh_stream(keep):
+    """A stream without a workspace, and its key."""
+    stream = torch.cuda.Stream()
+    key = (stream.device.index, stream.cuda_stream)
+    torch.cuda.synchronize()
+    keep.append(ops._workspaces.pop(key, None))  # an earlier test's graph may still hold it
+    return stream, key
+
+
+def _capture(t, stream):
+    """A graph of one call on t, captured on ``stream``, and the call's output."""
+    lens, cu, o = torch.tensor(t.lens, dtype=torch.int32, device="cuda"), _cu(t.new), torch.empty_like(t.q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        attention.attention_tree(t.q, t.kc, t.vc, t.table, lens, cu, t.mask, o)
+    return graph, o, (lens, cu)
+
+
+def test_graphs_captured_on_a_stream_that_never_ran(cuda_device):
+    """Two graphs on one such stream, the second with a larger workspace and replayed first; what
+    they wait on is zero before any of them runs, whatever the memory held."""
+    small, big = (Tree(n, new, 8, 2, 128, 16, torch.bfloat16, seed=45) for n, new in
+                  (([3000], [1]), ([500] * 9, [40] * 9)))
+    want = [t.run()[0] for t in (small, big)]
+    dirt = [torch.full((n << 20,), 255, dtype=torch.uint8, device="cuda") for n in (1, 2, 8, 64, 200)]
+    del dirt
+    keep = []
+    stream, key = _fresh_stream(keep)
+    first, o1, hold1 = _capture(small, stream)
+    assert not bool(ops._workspaces[key].any())
+    second, o2, hold2 = _capture(big, stream)
+    assert not bool(ops._workspaces[key].any())
+    for graph, o, expected in ((second, o2, want[1]), (first, o1, want[0]), (second, o2, want[1])):
+        o.fill_(float("nan"))
+        graph.replay()
+        assert torch.equal(o, expected)
+    ops.check_status()
+
+
+def test_a_replay_clears_nothing(cuda_device):
+    """The workspace's clearing is no part of a graph that was captured on a fresh stream."""
+    t = Tree([3000], [1], 8, 2, 128, 16, torch.bfloat16, seed=46)
+    want, _ = t.run()
+    keep = []
+    stream, key = _fresh_stream(keep)
+    lens, cu, o = torch.tensor(t.lens, dtype=torch.int32, device="cuda"), _cu(t.new), torch.empty_like(t.q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        ws = ops.workspace(96 << 20, cuda_device)  # more than the call takes
+        attention.attention_tree(t.q, t.kc, t.vc, t.table, lens, cu, t.mask, o)
+    assert ops._workspaces[key] is ws and not bool(ws.any())
+    ws[-1] = 7
+    graph.replay()
+    assert torch.equal(o, want) and int(ws[-1]) == 7
+    ws[-1] = 0
+    ops.check_status()
+
+
+FIRST_CALL = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+from gfx950_gluon_tutorials_b200 import attention, ops
+q, k, v = (torch.randn((50, h, 64), device="cuda").half() for h in (4, 2, 2))
+cu, o = torch.tensor([0, 20, 50], dtype=torch.int32, device="cuda"), torch.empty_like(q)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    attention.attention_prefill(q, k, v, cu, o)
+ops.check_status()
+ops.status_tensor(q.device).fill_(0x5000)  # as a kernel of another graph reports
+graph.replay()
+try:
+    ops.check_status()
+    raise SystemExit("the replay cleared the status word")
+except ops.B2GError as e:
+    assert e.code == 0x5000
+assert torch.equal(o, attention.attention_prefill(q, k, v, cu))
+ops.check_status()
+print("as expected")
+"""
+
+
+def test_first_call_of_a_process_is_captured(cuda_device):
+    """The status word too is there and clear before the first replay, and no replay clears it."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", FIRST_CALL, root], capture_output=True, text=True,
+                         timeout=300)
+    assert out.returncode == 0 and "as expected" in out.stdout, out.stdout + out.stderr
