@@ -219,8 +219,11 @@ __device__ __forceinline__ void tile_softmax(uint32_t s_col, uint32_t o_col, uin
   const float m_cand = mx * sl2;
   const bool move = m_cand > m_run + kRescaleLog2;
   const float m_new = move ? m_cand : m_run;
+  // One exponential for a row that moves: exact to fp32 rounding, since what it scales stays
+  // in the sum (poly_exp2's 7e-5 came out in the lse of a row with many keys just below the
+  // one that moved it). 0 where the maximum was -inf.
   float alpha = 1.0f;
-  if (move) alpha = poly_exp2(m_run - m_new);
+  if (move) alpha = fast_exp2(m_run - m_new);
   if (!first && __any_sync(0xffffffffu, move)) {
 #pragma unroll 1
     for (uint32_t d = 0; d < static_cast<uint32_t>(D); d += 16u) {

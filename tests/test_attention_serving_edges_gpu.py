@@ -12,7 +12,8 @@ import pytest
 import torch
 
 from gfx950_gluon_tutorials_b200 import attention, ops
-from test_attention_serving_gpu import DTYPES, Tree, _cu
+from oracle import serving
+from test_attention_serving_gpu import DTYPES, UNIT, Tree, _close, _cu, _gen, _np, _prefill, _rand
 
 pytestmark = pytest.mark.gpu
 
@@ -149,3 +150,36 @@ def test_first_call_of_a_process_is_captured(cuda_device):
     out = subprocess.run([sys.executable, "-c", FIRST_CALL, root], capture_output=True, text=True,
                          timeout=300)
     assert out.returncode == 0 and "as expected" in out.stdout, out.stdout + out.stderr
+
+
+# Many keys of score 0, then one 8 to 9.4 powers of two above: the maximum moves once, and what
+# was summed before still is most of the sum. A head for each of 16 such scores.
+LATE = dict(start=5.6, end=6.5, steps=16)
+
+
+def test_prefill_sum_before_a_late_maximum(cuda_device):
+    n, hq, d = 12001, 16, 64
+    q, k = (torch.zeros((n, h, d), dtype=torch.float16, device="cuda") for h in (hq, 1))
+    v = _rand(_gen(43), n, 1, d, dtype=torch.float16)
+    q[..., 0] = torch.linspace(**LATE, device="cuda").half()
+    k[-1, :, 0] = 1.0
+    o, lse = _prefill(q, k, v, [n], scale=1.0)
+    for h in range(hq):
+        ref = serving.attend(_np(q[-1:, h]), _np(k[:, 0]), _np(v[:, 0]), serving.causal(n)[-1:], 1.0,
+                             UNIT[q.dtype])
+        _close(_np(o[-1:, h]), _np(lse[h, -1:]), ref, f"head {h}")
+
+
+def test_tree_sum_before_a_late_maximum(cuda_device):
+    """Enough requests that a CTA holds most of a request's keys."""
+    keys, requests, new, hq, d, at = 3009, 150, 9, 16, 64, 2990
+    t = Tree([keys] * requests, [new] * requests, hq, 1, d, 64, torch.float16, seed=44, masked=False)
+    t.kc.zero_()
+    t.q.zero_()
+    t.q[..., 0] = torch.linspace(**LATE, device="cuda").half()
+    for r in range(requests):
+        t.k[r].zero_()
+        t.k[r][at, 0, 0] = 1.0
+        t.kc[t.table[r, at // 64], at % 64, 0, 0] = 1.0
+    o, lse = t.run(scale=1.0)
+    t.check(o, lse, scale=1.0, heads=range(hq), requests=[0, 1, 2, 74, 75, 149])
