@@ -145,18 +145,30 @@ struct PackedPlanParams {
 __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const PackedPlanParams p) {
   __shared__ int32_t level[2 * kPlanLevels];  // blocks of a level, then where they go
   __shared__ int32_t warp_sum[kPlanThreads / 32];
+  __shared__ int64_t warp_asked[kPlanThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   grid_launch_dependents();
   for (int i = threadIdx.x; i < 2 * kPlanLevels; i += kPlanThreads) level[i] = 0;
   __syncthreads();
   // a warp to a prompt, a lane to a block
+  int64_t asked = 0;
   for (int b = warp; b < p.prompts; b += kPlanThreads / 32) {
     int32_t begin;
     const int32_t rows = prompt_rows(p.cu, b, p.tokens, p.status, begin);
+    asked += (rows + p.block - 1) / p.block;
     for (int32_t row = lane * p.block; row < rows; row += 32 * p.block)
       atomicAdd(&level[block_level(row, rows, p.block)], 1);
   }
+  if (lane == 0) warp_asked[warp] = asked;
   __syncthreads();
+  // Offsets that decrease can ask for more blocks than the 32-bit sums below hold, whose
+  // places in the plan would then mean nothing: no block is run.
+  asked = 0;
+  for (int w = 0; w < kPlanThreads / 32; ++w) asked += warp_asked[w];
+  if (asked > INT_MAX) {
+    if (threadIdx.x == 0) *p.counts = make_int2(0, 0);
+    return;
+  }
   // exclusive sums over the levels, eight to a thread
   constexpr int kPer = 2 * kPlanLevels / kPlanThreads;
   int32_t mine[kPer], sum = 0;

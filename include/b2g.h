@@ -284,8 +284,9 @@ B2G_API int b2g_kv_write(const void* k, const void* v, void* k_cache, void* v_ca
  * (token, head) of q, k, v, o; the dim stride is 1, the others positive
  * multiples of 8, pointers 16-byte aligned. Prompts may be empty; rows of o and
  * lse past cu_seqlens[prompts] are not written. Offsets that decrease or pass
- * `tokens` are clamped and set B2G_STATUS_TOKENS. lse (nullable) is float
- * [heads_q][tokens]. Workspace as for the GEMMs, of at least
+ * `tokens` are clamped and set B2G_STATUS_TOKENS; rows that they name more than
+ * once may be left out. lse (nullable) is float [heads_q][tokens]. Workspace as
+ * for the GEMMs, of at least
  * b2g_attention_prefill_workspace_bytes(prompts, tokens, heads_q) bytes. */
 B2G_API size_t b2g_attention_prefill_workspace_bytes(int prompts, int64_t tokens, int heads_q);
 B2G_API int b2g_attention_prefill(const void* q, const void* k, const void* v, void* o,

@@ -11,9 +11,10 @@ import sys
 import pytest
 import torch
 
-from gfx950_gluon_tutorials_b200 import attention, ops
+from gfx950_gluon_tutorials_b200 import _lib, attention, ops
 from oracle import serving
-from test_attention_serving_gpu import DTYPES, UNIT, Tree, _close, _cu, _gen, _np, _prefill, _rand
+from test_attention_serving_gpu import (DTYPES, UNIT, Tree, _check_prefill, _close, _cu, _gen, _np,
+                                        _prefill, _rand)
 
 pytestmark = pytest.mark.gpu
 
@@ -183,3 +184,24 @@ def test_tree_sum_before_a_late_maximum(cuda_device):
         t.kc[t.table[r, at // 64], at % 64, 0, 0] = 1.0
     o, lse = t.run(scale=1.0)
     t.check(o, lse, scale=1.0, heads=range(hq), requests=[0, 1, 2, 74, 75, 149])
+
+
+def test_prefill_offsets_that_ask_for_too_much(cuda_device):
+    """Offsets that go back and forth over a million tokens until the blocks that they name pass
+    2^31 are reported, and no block of them is run; the next call is right."""
+    tokens, prompts = 1 << 20, (1 << 19) + 1024
+    cu = torch.zeros(prompts + 1, dtype=torch.int32, device="cuda")
+    cu[1::2] = tokens
+    assert (prompts // 2) * (tokens // 128) > 2 ** 31
+    q = torch.zeros((tokens, 2, 64), dtype=torch.float16, device="cuda")
+    k = torch.zeros((tokens, 1, 64), dtype=torch.float16, device="cuda")
+    o = torch.full_like(q, 7.0)
+    attention.attention_prefill(q, k, k, cu, o)
+    with pytest.raises(ops.B2GError) as e:
+        ops.check_status()
+    assert e.value.code == _lib.STATUS_TOKENS and bool((o == 7.0).all())
+    lens = [300] * 400  # enough blocks for the planning kernel
+    g = _gen(47)
+    q, k, v = (_rand(g, sum(lens), h, 64, dtype=torch.float16) for h in (2, 1, 1))
+    o, lse = _prefill(q, k, v, lens)
+    _check_prefill(q, k, v, lens, o, lse, 0.125, skip=range(3, 398))
