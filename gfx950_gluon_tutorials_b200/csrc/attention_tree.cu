@@ -96,6 +96,7 @@ struct alignas(64) TreeParams {
   int32_t mask_words, part_rows, requests;
   int32_t most;            // keys that a table has room for
   int32_t HQ, HK, G, tokens, page_size, num_pages;
+  int64_t most_units;      // units of a head that the call can ask for at most
   int32_t inject;          // test hook: joins wait for a part that nobody publishes
   float scale_log2;
   uint64_t timeout_ns;
@@ -222,6 +223,9 @@ __device__ __forceinline__ void find_share(const TreeParams& p, int64_t* sums, S
     if (i < warp) base += sums[i];
     upto += sums[i];
   }
+  // Offsets that decrease name rows more than once: what passes all that the call's shapes
+  // hold (hours of work from a few tokens) is not run. The status has been set above.
+  if (total > p.most_units) total = 0;
   const int64_t units = total * p.HK;
   const int64_t ctas = min(units, static_cast<int64_t>(gridDim.x));
   const int64_t u =
@@ -1235,6 +1239,10 @@ extern "C" int b2g_attention_tree(const void* q, const void* k_cache, const void
   prm.requests = requests;
   prm.most = static_cast<int32_t>(
       std::min<int64_t>(static_cast<int64_t>(max_pages) * page_size, INT_MAX - 256));
+  // a block for every 256 rows, a ragged one for each request, each with all tiles
+  prm.most_units =
+      (tokens * group / 256 + std::min<int64_t>(requests, tokens)) *
+      (std::max<int64_t>((static_cast<int64_t>(prm.most) + 127) / 128, 1) + kBlockCost);
   prm.part = reinterpret_cast<float*>(ws + wl.part);
   prm.part_ml = reinterpret_cast<float2*>(ws + wl.part_ml);
   prm.part_rows = wl.part_rows;

@@ -308,8 +308,10 @@ B2G_API int b2g_attention_prefill(const void* q, const void* k, const void* v, v
  * 64 or a multiple of 128. Keys in a page past seq_lens[r] are never used,
  * whatever they hold. A table entry outside [0, num_pages) reads as zero keys
  * and values and sets B2G_STATUS_PAGE_TABLE, as does a request longer than its
- * table. lse (nullable) is float [heads_q][tokens]. Workspace as for the GEMMs,
- * of at least b2g_attention_tree_workspace_bytes(...) bytes. */
+ * table. Offsets that decrease or pass `tokens` are clamped and set
+ * B2G_STATUS_TOKENS; nothing is run when they ask for more than the shapes hold.
+ * lse (nullable) is float [heads_q][tokens]. Workspace as for the GEMMs, of at
+ * least b2g_attention_tree_workspace_bytes(...) bytes. */
 B2G_API size_t b2g_attention_tree_workspace_bytes(int requests, int64_t tokens, int heads_q,
                                                   int heads_k, int head_dim);
 B2G_API int b2g_attention_tree(const void* q, const void* k_cache, const void* v_cache, void* o,

@@ -205,3 +205,26 @@ def test_prefill_offsets_that_ask_for_too_much(cuda_device):
     q, k, v = (_rand(g, sum(lens), h, 64, dtype=torch.float16) for h in (2, 1, 1))
     o, lse = _prefill(q, k, v, lens)
     _check_prefill(q, k, v, lens, o, lse, 0.125, skip=range(3, 398))
+
+
+def test_tree_offsets_that_ask_for_too_much(cuda_device):
+    """Offsets that decrease are reported; those that name every row for every second of many
+    requests are not run at all. The next call is right."""
+    tokens, requests = 4096, 4096
+    t = Tree([100], [3], 2, 2, 64, 16, torch.float16, seed=48)
+    q = torch.zeros((tokens, 2, 64), dtype=torch.float16, device="cuda")
+    lens = torch.full((requests,), 100, dtype=torch.int32, device="cuda")
+    table = t.table.expand(requests, -1).contiguous()
+    for cu, run in ((torch.arange(requests + 1, device="cuda").int(), True),
+                    (torch.arange(requests + 1, device="cuda").int() % 2 * tokens, False)):
+        o = torch.full_like(q, 7.0)
+        attention.attention_tree(q, t.kc, t.vc, table, lens, cu, None, o)
+        if run:
+            ops.check_status()
+            assert not bool((o == 7.0).all(-1).any())
+        else:
+            with pytest.raises(ops.B2GError) as e:
+                ops.check_status()
+            assert e.value.code == _lib.STATUS_TOKENS and bool((o == 7.0).all())
+    o, lse = t.run()
+    t.check(o, lse)
