@@ -5,6 +5,7 @@ batches large enough for every way of planning the work. Against float64, as the
 from __future__ import annotations
 
 import os
+import random
 import subprocess
 import sys
 
@@ -228,3 +229,51 @@ def test_tree_offsets_that_ask_for_too_much(cuda_device):
             assert e.value.code == _lib.STATUS_TOKENS and bool((o == 7.0).all())
     o, lse = t.run()
     t.check(o, lse)
+
+
+@pytest.mark.parametrize("requests,hq,hk,d", [(321, 4, 2, 64), (700, 4, 2, 64), (1000, 8, 1, 128)])
+def test_tree_more_requests_than_threads(cuda_device, requests, hq, hk, d):
+    """More requests than a CTA has threads: shares are found in several rounds, across runs of
+    requests without new tokens that span the rounds' borders."""
+    rng = random.Random(requests)
+    lens = [rng.choice([1, 5, 64, 129, 300]) for _ in range(requests)]
+    new = [min(n, rng.choice([0, 1, 1, 3, 9])) for n in lens]
+    for r in (*range(300, min(340, requests - 1)), *range(630, min(660, requests - 1))):
+        new[r] = 0
+    lens[-1] = new[-1] = 1
+    t = Tree(lens, new, hq, hk, d, 16, torch.bfloat16, seed=requests)
+    o, lse = t.run()
+    t.check(o, lse, heads=[0, hq - 1])
+
+
+def test_tree_no_request_but_the_last(cuda_device):
+    """Rounds of requests without any work before the one that has some."""
+    t = Tree([0] * 650 + [2000], [0] * 650 + [5], 4, 2, 64, 16, torch.float16, seed=49)
+    o, lse = t.run()
+    t.check(o, lse)
+
+
+@pytest.mark.parametrize("hq,hk,d", [(3, 3, 64), (10, 2, 128), (1, 1, 128), (4, 2, 64)])
+def test_prefill_planned_blocks(cuda_device, hq, hk, d):
+    """Enough blocks for the planning kernel, where an odd number of query heads per key/value
+    head takes two row tiles at a time and a ragged one by pairs of heads."""
+    rng = random.Random(hq)
+    lens = [rng.choice([1, 100, 128, 129, 255, 256, 257, 400, 513, 700]) for _ in range(180)]
+    g, t = _gen(hq), sum(lens)
+    block = 256 if hq // hk % 2 else 128
+    assert sum(-(-n // block) for n in lens) > 256
+    q, k, v = (_rand(g, t, h, d, dtype=torch.bfloat16) for h in (hq, hk, hk))
+    o, lse = _prefill(q, k, v, lens)
+    _check_prefill(q, k, v, lens, o, lse, d ** -0.5, skip=[b for b in range(180) if b % 6])
+
+
+@pytest.mark.parametrize("hq,hk", [(1, 1), (4, 2)])
+def test_prefill_more_prompts_than_threads(cuda_device, hq, hk):
+    """Hundreds of prompts, nearly all of them empty."""
+    lens = [0] * 500
+    for b, n in ((0, 3), (7, 300), (319, 1), (320, 129), (321, 256), (498, 40)):
+        lens[b] = n
+    g, t = _gen(50), sum(lens)
+    q, k, v = (_rand(g, t, h, 64, dtype=torch.float16) for h in (hq, hk, hk))
+    o, lse = _prefill(q, k, v, lens)
+    _check_prefill(q, k, v, lens, o, lse, 0.125)
