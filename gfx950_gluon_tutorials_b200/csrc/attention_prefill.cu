@@ -24,8 +24,9 @@
 // What bounds it: the two products and the exponentials of a tile, as in
 // attention.cu, and for short prompts the hand-over from item to item. 12031 tokens,
 // 32 heads over 8, 128: 945-1078 us (1250-1100 TFLOPS; the power cap moves it, 1689 is
-// the measured rate of a plain product); 24 prompts of 1 to 1100 tokens 129-145 us; 96
-// of up to 300, 24 heads of 64: 74-76 us (1.75 TB/s of what has to move). Measured and
+// the measured rate of a plain product); 24 prompts of 1 to 1100 tokens 144 us per call, 128
+// in a replayed graph whose inputs stay in L2; 96 of up to 300, 24 heads of 64: 73-74 us
+// either way (1.8 TB/s of what has to move). Measured and
 // not kept: half of a row's columns to each of two threads (16 softmax warps) 1213-1341
 // us for the first; one wait for all of P instead of one for each half, 5-8 % slower; a
 // quarter of the exponentials as poly_exp2, no gain at 128 and 9 % at 64, for a sum of

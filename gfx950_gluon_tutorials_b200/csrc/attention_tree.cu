@@ -32,12 +32,17 @@
 // with its own maximum, sum and O; they meet in shared memory at the end of the
 // block, together with the two warpgroups'.
 //
-// Measured: 64 requests of up to 8192 keys, 32 heads over 8, one token each: 288-303 us,
-// 5.5-5.7 TB/s; 16 requests of up to 5000 keys with trees of up to 64 drafts 116 us; two
-// of 100003 and 81102 keys with up to 12 drafts, 16 heads over 2, 67.5 us; one of 777
-// keys, one token, 16.7 us. Pages of 16 tokens cost the decode a fifth: a box of 2 KB
-// takes about 100 cycles to issue and there are 32 to a tile. Issued from one lane of a
-// converged warp they cost less (344 -> 313 us) but the few boxes of larger pages more
+// Measured, per call back to back (and in a replayed graph, on the GPU alone): 64 requests
+// of up to 8192 keys, 32 heads over 8 of 128, one token each: 304-321 us, 5.1-5.4 TB/s
+// (285-288); 384 of up to 2000 keys 580 us, 4.1 TB/s (550); 16 requests of up to 5000 keys
+// with trees of up to 64 drafts 116 us (112-116, up to 140 after other work); two of
+// 100003 and 81102 keys with up to 12 drafts, 16 heads over 2, 69 us (67); one of 777 keys,
+// one token, 18.4 us (16.5-21); 2048 new tokens over 8192, 418 us, 740 TFLOPS (414); 256 of
+// up to 200 keys 127 us (125), which is beginning blocks. Heads of 64: the decode 234 us
+// (224), the drafts 96, the long two 50.
+// Pages of 16 tokens cost the decode a fifth: a box of 2 KB takes about 100 cycles to issue
+// and there are 32 to a tile. Issued from one lane of a converged warp they cost less on
+// the GPU (344 -> 313 us) but the few boxes of larger pages more
 // (288 -> 308), and code for both slowed either. Asking tiles into L2 ahead of the ring
 // adds boxes and lost 3-25 %. A warp that fetches the next block's Q during the joins
 // changed nothing.
@@ -45,7 +50,8 @@
 // Pages: a tile is gathered by one TMA box per page and 64-element slab (a page
 // of 128 tokens or more is one box), each lane of the producer warp issuing one.
 // Keys past the request's length are loaded from past the last page, which fills
-// zeros. Values that are not finite are handled as in attention.cu.
+// zeros. Values that are not finite are handled as in attention_prefill.cu, and scores of
+// NaN reach their row however its keys are split (see join_parts).
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -102,8 +108,14 @@ struct alignas(64) TreeParams {
   uint64_t timeout_ns;
 };
 
-// Tiles that beginning a block counts as in the cut of the shares. Interleaved, for 0 / 5 /
-// 8: 16 drafted trees 124-132 / 117 / 116 us, two long caches 72-76 / 72 / 68, decode alike.
+// Tiles that beginning a block counts as in the cut of the shares. What it costs depends on
+// rows, pages and head dim, but one count serves them. Interleaved, for 0 / 4 / 8 / 16, us:
+//   heads of 128: 16 drafted trees 127 / 117 / 116 / 112, two long caches 77 / 72 / 69 / 62,
+//     384 requests of up to 2000 keys 591 / 587 / 581 / 587, 256 of up to 200 keys 155 / 129 /
+//     127 / 124, 64 of up to 600 with 8 drafts 89 / 72 / 73 / 75, 2048 new tokens over 8192
+//     415 / 415 / 418 / 423
+//   heads of 64: the trees 101 / 99 / 96 / 104, the long caches 55 / 50 / 50 / 50, 64 requests
+//     of up to 8192 keys 238 / 234 / 234 / 235
 constexpr int32_t kBlockCost = 8;
 
 template <int D>
@@ -379,7 +391,7 @@ __device__ __forceinline__ uint32_t seen_bits(const TreeParams& p, const TreeEnt
 }
 
 // Adds to n values of a row of O (of new token i, from dim d0 on) what is not
-// finite among the values that the token sees; see attention.cu.
+// finite among the values that the token sees; see attention_prefill.cu.
 template <int D, typename T, typename OutT>
 __device__ __noinline__ void add_odd_cache_values(const TreeParams& p, const Segment& s, int32_t i,
                                                   int32_t d0, int32_t n, OutT* out) {
@@ -1081,6 +1093,9 @@ __global__ void __launch_bounds__(TreePlan<D>::kThreads, 1)
       if (*abort_flag != 0u) continue;
       const int32_t k = me - b.owner, wi = static_cast<int32_t>(w8), ln = static_cast<int32_t>(lane);
       float* sums = reinterpret_cast<float*>(smem + TP::kJoinOff);
+      // Few parts: more columns to a thread instead of loads of parts that are not there.
+      // With the last form alone, 16 drafted trees take 154 us instead of 116, 2048 new
+      // tokens over 8192 461 instead of 418; two long caches, 74 parts a block, are alike.
       const int32_t parts = b.parts * b.each;
       if (parts <= 2)
         join_parts<D, kBF16, 4, 2>(p, b, k, wi, ln, sums);

@@ -26,7 +26,6 @@ from . import _lib
 from .ops import _require_cuda, _stream_handle, status_tensor
 
 _DT = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
-MAX_REQUESTS = 8192
 _I64x10 = ctypes.c_int64 * 10
 _ONE = torch.Size([1])
 
@@ -65,7 +64,8 @@ def map_step(cached_lens: torch.Tensor, new_lens: torch.Tensor, page_counts: tor
 
     When the list runs out, the missing table entries and slots are -1 and the
     returned ``num_free`` is minus the number of missing pages. All lengths,
-    counts and tables are int32 CUDA tensors, ``num_free`` of shape (1,)."""
+    counts and tables are int32 CUDA tensors, ``num_free`` of shape (1,). At most
+    8192 requests."""
     dev = _require_cuda(cached_lens, new_lens, page_counts, block_tables, free_pages, num_free)
     i32 = torch.int32
     if block_tables.dtype is not i32 or len(block_tables.shape) != 2:
